@@ -10,7 +10,8 @@ from __future__ import annotations
 
 import ctypes
 import threading
-from ctypes import POINTER, c_bool, c_double, c_float, c_int, c_int64, c_size_t, c_uint, c_void_p
+from ctypes import (POINTER, c_bool, c_double, c_float, c_int, c_int64, c_size_t, c_uint,
+                    c_uint64, c_void_p)
 from pathlib import Path
 
 LIBRARY = Path(__file__).resolve().with_name("libclad3dgs_b200.so")
@@ -112,6 +113,8 @@ _SIGNATURES = {
     "clad3dgs_ipc_free": (c_int, [_P]),
     "clad3dgs_ipc_open": (c_int, [POINTER(ctypes.c_ubyte), POINTER(c_void_p)]),
     "clad3dgs_ipc_close": (c_int, [_P]),
+    "clad3dgs_dropout": (c_int, [c_int, c_int64, c_int64, _P, c_int64, _P, c_int64, c_double,
+                                 c_uint64, c_uint64, _P, c_int, _P]),
 }
 
 _lock = threading.Lock()

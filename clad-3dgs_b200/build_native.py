@@ -36,6 +36,7 @@ FLAGS = {
     "rasterizer.cu": [],
     "sh_backward.cu": ["-fmad=false"],
     "train_step.cu": ["-fmad=false"],
+    "dropout.cu": [],
 }
 
 

@@ -1,0 +1,68 @@
+// The keep/drop decisions of the dropout, drawn from a counter and never stored.
+//
+// Element e of a call keeps its value iff word e % 4 of Philox4x32-10 at the
+// counter (e / 4 low, e / 4 high, offset low, offset high) under the key
+// (seed low, seed high) is at least floor(p * 2^32). The generator is the one
+// of Salmon, Moraes, Dror and Shaw, "Parallel random numbers: as easy as
+// 1, 2, 3" (SC'11): ten rounds of two 32 x 32 -> 64 bit products, their high
+// halves mixed with the other words and a key that grows by a constant every
+// round. One call serves four elements; any kernel that knows an element's
+// number finds its decision again, so the backward pass needs no mask.
+#pragma once
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace clad3dgs {
+
+// One dropout as a kernel argument: kept iff word >= limit, for p < 1; `none`
+// keeps nothing (p = 1, whose limit does not fit a word).
+struct CounterMask {
+  uint32_t key0, key1;
+  unsigned long long offset;
+  const long long* offset_device;  // nullable: added to offset by the kernel
+  uint32_t limit;
+  bool none;
+
+  __device__ __forceinline__ bool keeps(uint32_t word) const { return word >= limit && !none; }
+};
+
+inline CounterMask counter_mask(double p, uint64_t seed, uint64_t offset,
+                                const long long* offset_device) {
+  CounterMask m;
+  m.key0 = uint32_t(seed);
+  m.key1 = uint32_t(seed >> 32);
+  m.offset = offset;
+  m.offset_device = offset_device;
+  m.none = p >= 1.0;
+  m.limit = m.none ? 0 : uint32_t(p * 4294967296.0);
+  return m;
+}
+
+__device__ __forceinline__ unsigned long long mask_offset(const CounterMask& m) {
+  return m.offset + (m.offset_device ? (unsigned long long)*m.offset_device : 0ull);
+}
+
+__device__ __forceinline__ uint4 mask_words(const CounterMask& m, unsigned long long offset,
+                                            unsigned long long block) {
+  uint32_t c0 = uint32_t(block), c1 = uint32_t(block >> 32), c2 = uint32_t(offset),
+           c3 = uint32_t(offset >> 32), k0 = m.key0, k1 = m.key1;
+#pragma unroll
+  for (int r = 0; r < 10; ++r) {
+    const unsigned long long a = (unsigned long long)0xD2511F53u * c0;
+    const unsigned long long b = (unsigned long long)0xCD9E8D57u * c2;
+    c0 = uint32_t(b >> 32) ^ c1 ^ k0;
+    c1 = uint32_t(b);
+    c2 = uint32_t(a >> 32) ^ c3 ^ k1;
+    c3 = uint32_t(a);
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  return make_uint4(c0, c1, c2, c3);
+}
+
+__device__ __forceinline__ uint32_t word_of(const uint4& w, unsigned j) {
+  return j == 0 ? w.x : j == 1 ? w.y : j == 2 ? w.z : w.w;
+}
+
+}  // namespace clad3dgs

@@ -1,0 +1,129 @@
+"""Dropout from a counter-based generator, with a mask that is never stored.
+
+`dropout(x, p, seed, offset)` keeps element e of x (counted in row-major
+order) iff the e-th word that Philox4x32-10 gives for (seed, offset) is at
+least floor(p * 2^32), scales what it keeps by 1 / (1 - p) and sets the rest
+to zero. The same numbers always give the same decisions, whatever x's layout
+or type, so the backward pass draws them again instead of reading a mask; a
+program picks a new `offset` for every call (a step counter, say) under one
+`seed`. `rows=True` decides once for each row (all of the last dimension):
+Gaussians or tokens are dropped whole.
+
+`offset` may be a one-element int64 CUDA tensor, read when the kernel runs: a
+captured graph then draws anew at each replay once the program has advanced
+it. It must not change between a forward pass and its backward pass (autograd
+checks the tensor's version).
+
+float32, float16 and bfloat16; inputs may have any layout, outputs are
+contiguous. Kernels launch on the current stream of x's device. Bad arguments
+raise RuntimeError before anything is written.
+"""
+
+from __future__ import annotations
+
+import torch
+
+import _native as native
+
+TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+WORD = 2 ** 64
+
+
+def _require(condition, message):
+    if not condition:
+        raise RuntimeError(message)
+
+
+def check_draw(p, seed, offset, device):
+    """Checks a dropout's numbers; returns (offset as an int, address of the
+    device offset or None)."""
+    _require(isinstance(p, (int, float)) and 0.0 <= p <= 1.0, "p must lie in [0, 1]")
+    _require(isinstance(seed, int) and 0 <= seed < WORD, "seed must be an integer in [0, 2^64)")
+    if isinstance(offset, torch.Tensor):
+        _require(offset.device == device and offset.dtype == torch.int64
+                 and offset.numel() == 1, "a tensor offset must be one int64 on the input's device")
+        return 0, offset.data_ptr()
+    _require(isinstance(offset, int) and 0 <= offset < WORD,
+             "offset must be an integer in [0, 2^64) or a CUDA tensor")
+    return offset, None
+
+
+def row_layout(x):
+    """x as rows of its last dimension: (x, rows, width, row stride), packed
+    first unless it is contiguous or a 2-D tensor with unit column stride."""
+    width = x.shape[-1] if x.dim() else 1
+    if x.numel() == 0:
+        return x, 0, width, width
+    if not x.is_contiguous():
+        if x.dim() == 2 and x.stride(1) == 1:
+            return x, x.shape[0], width, x.stride(0)
+        x = x.contiguous()
+    return x, x.numel() // width, width, width
+
+
+def on_device(device, call):
+    """call() with `device` current."""
+    if device.index == torch.cuda.current_device():
+        return call()
+    with torch.cuda.device(device):
+        return call()
+
+
+def _launch(x, p, seed, offset, rows, out):
+    number, address = check_draw(p, seed, offset, x.device)
+    x, count, width, stride = row_layout(x)
+    if count == 0:
+        return out
+    on_device(x.device, lambda: native.check(native.library().clad3dgs_dropout(
+        TYPES[x.dtype], count, width, x.data_ptr(), stride, out.data_ptr(), width, p, seed,
+        number, address, int(rows), native.stream_handle()), "dropout"))
+    return out
+
+
+def apply(x, p, seed, offset=0, *, rows=False, out=None):
+    """The dropout without autograd. `out`: a contiguous tensor like x to write
+    into; x itself (contiguous) for a call in place."""
+    _require(x.is_cuda, "dropout needs a CUDA tensor")
+    _require(x.dtype in TYPES, "dropout takes float32, float16 or bfloat16")
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    else:
+        _require(out.device == x.device and out.dtype == x.dtype and out.shape == x.shape
+                 and out.is_contiguous(), "out must be a contiguous tensor like x")
+        same = out.data_ptr() == x.data_ptr() and x.is_contiguous()
+        _require(same or not _overlap(x, out), "out may be x itself, but not overlap it otherwise")
+    return _launch(x, p, seed, offset, rows, out)
+
+
+def _overlap(x, out):
+    if x.numel() == 0:
+        return False
+    first = x.data_ptr()
+    last = first + x.element_size() * (1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride())))
+    return first < out.data_ptr() + out.numel() * out.element_size() and out.data_ptr() < last
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, p, seed, offset, rows):
+        ctx.numbers = p, seed, rows
+        if isinstance(offset, torch.Tensor):
+            ctx.save_for_backward(offset)
+            ctx.offset = None
+        else:
+            ctx.offset = offset
+        return apply(x, p, seed, offset, rows=rows)
+
+    @staticmethod
+    def backward(ctx, grad):
+        p, seed, rows = ctx.numbers
+        offset = ctx.saved_tensors[0] if ctx.offset is None else ctx.offset
+        return dropout(grad, p, seed, offset, rows=rows), None, None, None, None
+
+
+def dropout(x, p, seed, offset=0, *, rows=False):
+    """x with a share p of its elements (rows=True: of its rows) set to zero and
+    the others scaled by 1 / (1 - p); differentiable any number of times."""
+    if x.requires_grad and torch.is_grad_enabled():
+        return _Dropout.apply(x, p, seed, offset, rows)
+    return apply(x, p, seed, offset, rows=rows)

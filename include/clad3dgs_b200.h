@@ -478,6 +478,29 @@ int clad3dgs_ipc_free(void* ptr);
 int clad3dgs_ipc_open(const unsigned char* handle, void** ptr);
 int clad3dgs_ipc_close(void* ptr);
 
+/* ===================== table operators and dropout ===================== */
+/* No counterpart in the reference. Features that many Gaussians (or tokens)
+ * share: rows of a table looked up by index, their gradients, and dropout. */
+
+/* Element types (arithmetic is in 32-bit floats for all three). */
+#define CLAD3DGS_F32 0
+#define CLAD3DGS_F16 1
+#define CLAD3DGS_BF16 2
+
+/* Dropout of a [rows][width] array (row strides in elements, unit column
+ * stride; y == x with equal strides is allowed, other overlaps are not):
+ * y[e] = x[e] / (1 - p) where element e = row * width + column is kept, else
+ * +0. Kept iff word e % 4 of Philox4x32-10 at counter (e / 4 low, e / 4 high,
+ * offset low, offset high) and key (seed low, seed high) is at least
+ * floor(p * 2^32); with by_row != 0 the row number stands for e, so rows are
+ * kept or dropped whole. offset_device (nullable) points to one device integer
+ * that is added to offset when the kernel runs (a captured graph draws anew at
+ * every replay when the program advances it). The adjoint is the same call on
+ * the gradient. */
+int clad3dgs_dropout(int type, int64_t rows, int64_t width, const void* x, int64_t x_stride,
+                     void* y, int64_t y_stride, double p, uint64_t seed, uint64_t offset,
+                     const int64_t* offset_device, int by_row, cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
