@@ -115,6 +115,20 @@ _SIGNATURES = {
     "clad3dgs_ipc_close": (c_int, [_P]),
     "clad3dgs_dropout": (c_int, [c_int, c_int64, c_int64, _P, c_int64, _P, c_int64, c_double,
                                  c_uint64, c_uint64, _P, c_int, _P]),
+    "clad3dgs_token_order_workspace": (c_size_t, [c_int64, c_int64]),
+    "clad3dgs_token_order": (c_int, [c_int64, c_int64, _P, c_int, c_int, c_int64, _P, _P,
+                                     c_size_t, _P]),
+    "clad3dgs_embedding_lookup": (c_int, [c_int, c_int64, c_int64, c_int64, _P, c_int64, _P,
+                                          c_int, c_int, c_int64, c_double, c_double, c_uint64,
+                                          c_uint64, _P, _P, _P]),
+    "clad3dgs_embedding_workspace": (c_size_t, [c_int64, c_int64]),
+    "clad3dgs_embedding_gradient": (c_int, [c_int, c_int64, c_int64, c_int64, _P, c_int64, _P,
+                                            c_double, c_double, c_uint64, c_uint64, _P, _P, _P,
+                                            c_size_t, _P]),
+    "clad3dgs_embedding_consume_torch_adam": (c_int, [c_int, c_int64, c_int64, c_int64, _P,
+                                                      c_int64, _P, c_double, c_double, c_uint64,
+                                                      c_uint64, _P, _P, _P, _P, c_double,
+                                                      TorchAdamConfig, _P, c_size_t, _P]),
 }
 
 _lock = threading.Lock()

@@ -37,6 +37,7 @@ FLAGS = {
     "sh_backward.cu": ["-fmad=false"],
     "train_step.cu": ["-fmad=false"],
     "dropout.cu": [],
+    "embedding.cu": [],
 }
 
 

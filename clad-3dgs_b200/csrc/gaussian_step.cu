@@ -781,6 +781,8 @@ __global__ void quaternion_kernel(long long n, const float* __restrict__ q,
 // ---------------------------------------------------------------------------
 // Host side.
 
+cudaError_t token_fault(bool clear, unsigned* word);  // embedding.cu
+
 thread_local std::string t_last_error;
 
 int fail(int code, const std::string& message) {
@@ -1088,9 +1090,13 @@ extern "C" int clad3dgs_fault_status(int clear, unsigned int* fault_word) {
     e = cudaMemcpyToSymbol(g_fault_word, &zero, sizeof(zero));
     if (e != cudaSuccess) return status_of(e, "clearing the fault word");
   }
-  if (fault_word) *fault_word = word;
-  return word ? fail(CLAD3DGS_DEVICE_FAULT, "a pipeline wait timed out")
-              : CLAD3DGS_OK;
+  unsigned int token_word = 0;
+  e = token_fault(clear != 0, &token_word);
+  if (e != cudaSuccess) return status_of(e, "reading the token fault word");
+  if (fault_word) *fault_word = word | token_word;
+  if (word) return fail(CLAD3DGS_DEVICE_FAULT, "a pipeline wait timed out");
+  return token_word ? fail(CLAD3DGS_DEVICE_FAULT, "a token's index lay outside its table")
+                    : CLAD3DGS_OK;
 }
 
 extern "C" int clad3dgs_sh_consume_split_torch_adam(

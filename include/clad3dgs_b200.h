@@ -128,7 +128,8 @@ int clad3dgs_describe(int* sm_count, int* tile_gaussians, int* sh_stages,
                       int* fused_stages);
 
 /* Reads (and clears if clear != 0) the device fault word that bounded waits
- * set when a pipeline barrier timed out. 0 means no fault. Synchronises. */
+ * set when a pipeline barrier timed out, and the table operators (bit 256) when
+ * a token's index lay outside its table. 0 means no fault. Synchronises. */
 int clad3dgs_fault_status(int clear, unsigned int* fault_word);
 
 /* Same as sh_consumer_split_torch_adam with an explicit stream. */
@@ -500,6 +501,55 @@ int clad3dgs_ipc_close(void* ptr);
 int clad3dgs_dropout(int type, int64_t rows, int64_t width, const void* x, int64_t x_stride,
                      void* y, int64_t y_stride, double p, uint64_t seed, uint64_t offset,
                      const int64_t* offset_device, int by_row, cudaStream_t stream);
+
+/* Stable order of n tokens by the row of a table they name: order[n][2] =
+ * (row, position), sorted by row, positions ascending within a row; tokens
+ * that name none of the `rows` rows come last with row number `rows`. index is
+ * int32 or int64 (index_bits); an index equal to `padding` (has_padding != 0)
+ * names no row, nor does one outside [0, rows), which also sets a bit of the
+ * fault word (clad3dgs_fault_status). n and rows below 2^31. workspace:
+ * clad3dgs_token_order_workspace bytes, 256-byte aligned, free again when the
+ * call's work on the stream is done. */
+size_t clad3dgs_token_order_workspace(int64_t n, int64_t rows);
+int clad3dgs_token_order(int64_t n, int64_t rows, const void* index, int index_bits,
+                         int has_padding, int64_t padding, uint32_t* order, void* workspace,
+                         size_t workspace_bytes, cudaStream_t stream);
+
+/* Rows of a table [rows][width] (row stride in elements) looked up by n
+ * tokens into out [n][width]: out[i] = scale * table[index[i]], with the dropout
+ * of clad3dgs_dropout over out's elements in the same pass if p > 0 (element
+ * i * width + d). Tokens that name no row (as in clad3dgs_token_order) give
+ * zeros. */
+int clad3dgs_embedding_lookup(int type, int64_t n, int64_t rows, int64_t width,
+                              const void* table, int64_t table_stride, const void* index,
+                              int index_bits, int has_padding, int64_t padding, double scale,
+                              double p, uint64_t seed, uint64_t offset,
+                              const int64_t* offset_device, void* out, cudaStream_t stream);
+
+/* The lookup's adjoint: out[k] = scale * sum over tokens i of row k of
+ * grad[i] (through the dropout of the same p, seed and offset), [rows][width]
+ * of grad's type, every row written (zeros where no token names it). grad
+ * [n][width] with a row stride in elements; order from clad3dgs_token_order of
+ * the same n and rows. Sums are 32-bit floats in an order that depends on
+ * the sizes alone. workspace: clad3dgs_embedding_workspace bytes, 16-byte
+ * aligned. */
+size_t clad3dgs_embedding_workspace(int64_t n, int64_t width);
+int clad3dgs_embedding_gradient(int type, int64_t n, int64_t rows, int64_t width,
+                                const void* grad, int64_t grad_stride, const uint32_t* order,
+                                double scale, double p, uint64_t seed, uint64_t offset,
+                                const int64_t* offset_device, void* out, void* workspace,
+                                size_t workspace_bytes, cudaStream_t stream);
+
+/* The adjoint handed straight to torch-fused Adam (rate, bias corrections as
+ * elsewhere in this header): table and both moments [rows][width], float,
+ * updated in place; the table's gradient is never written. Dense: rows that no
+ * token names are updated with a gradient of zero. The arrays must be disjoint
+ * from each other and from grad. */
+int clad3dgs_embedding_consume_torch_adam(
+    int type, int64_t n, int64_t rows, int64_t width, const void* grad, int64_t grad_stride,
+    const uint32_t* order, double scale, double p, uint64_t seed, uint64_t offset,
+    const int64_t* offset_device, float* table, float* first, float* second, double rate,
+    TorchAdamConfig config, void* workspace, size_t workspace_bytes, cudaStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,515 @@
+"""Table operators on the GPU against the definition in 64 bits.
+
+Tolerances count roundings. A lookup makes one product with a factor rounded to
+32 bits (2 x 2^-24) and one conversion (half a step of the type). A row's
+gradient adds m terms in 32 bits in some order: at most m roundings of partial
+sums, each at most 2^-24 of the sum of the terms' sizes, then the factor as
+above and one conversion.
+"""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import draws
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+SEED, OFFSET = 0xFEDCBA9876543210, 2 ** 35 + 7
+U = 2.0 ** -24
+
+
+def _step(dtype):
+    """Half a step of the type relative to a value, and below its normal range."""
+    return (0.0, 0.0) if dtype == torch.float32 else (torch.finfo(dtype).eps / 2, 2.0 ** -25)
+
+
+def _tokens(kind, n, rows, rng):
+    if kind == "uniform":
+        return rng.integers(0, rows, n)
+    if kind == "skewed":  # a few rows far more used than the rest
+        return np.minimum((np.exp(rng.random(n) * math.log(rows + 1)) - 1).astype(np.int64), rows - 1)
+    if kind == "same":
+        return np.full(n, rows // 2)
+    if kind == "sorted":
+        return np.sort(rng.integers(0, rows, n))
+    assert kind == "distinct"
+    return rng.permutation(max(n, rows))[:n] % rows
+
+
+def _case(n, rows, width, dtype, cuda, *, kind="uniform", bits=64, padding=False, seed=0):
+    rng = np.random.default_rng(seed)
+    index = _tokens(kind, n, rows, rng)
+    if padding:
+        index = np.where(rng.random(n) < 0.2, -1, index)
+    index = torch.from_numpy(index.astype(np.int64)).to(torch.int64 if bits == 64 else torch.int32)
+    table = torch.from_numpy(rng.standard_normal((rows, width))).to(dtype)
+    grad = torch.from_numpy(rng.standard_normal((n, width))).to(dtype)
+    return table.to(cuda), index.to(cuda), grad.to(cuda)
+
+
+def _check_lookup(got, table, index, scale, p, dtype, offset=OFFSET):
+    t, i = table.double().cpu().numpy(), index.cpu().numpy().reshape(-1)
+    want = np.where((i >= 0)[:, None], t[np.maximum(i, 0)], 0.0) * scale
+    if p > 0:
+        want = want * draws.weight(want.shape, p, SEED, offset)
+    half, tiny = _step(dtype)
+    got = got.double().cpu().numpy().reshape(want.shape)
+    assert (np.abs(got - want) <= np.abs(want) * (half + 2.01 * U) + tiny).all()
+
+
+def _check_gradient(got, grad, index, rows, scale, p, dtype, offset=OFFSET):
+    g, i = grad.double().cpu().numpy(), index.cpu().numpy().reshape(-1)
+    g = g.reshape(len(i), -1) * scale
+    if p > 0:
+        g = g * draws.weight(g.shape, p, SEED, offset)
+    want, size = np.zeros((rows, g.shape[1])), np.zeros((rows, g.shape[1]))
+    real = i >= 0
+    np.add.at(want, i[real], g[real])
+    np.add.at(size, i[real], np.abs(g[real]))
+    terms = np.bincount(i[real], minlength=rows)[:, None]
+    half, tiny = _step(dtype)
+    got = got.double().cpu().numpy()
+    assert got.shape == want.shape
+    assert not got[terms[:, 0] == 0].any()
+    limit = size * (terms + 2.01) * U + np.abs(want) * half + tiny * (terms > 0)
+    assert (np.abs(got - want) <= limit).all(), np.max(np.abs(got - want) - limit)
+
+
+SIZES = [(1, 1, 1), (1, 5, 2048), (2, 1, 3), (7, 3, 45), (31, 100, 48), (32, 2, 16), (33, 1000, 77),
+         (257, 9, 130), (1000, 64, 300), (4097, 5003, 33), (3000, 1, 8), (20_011, 700, 48)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,rows,width", SIZES)
+@pytest.mark.parametrize("p", [0.0, 0.3])
+def test_lookup(cuda, dtype, n, rows, width, p):
+    import embedding
+
+    for bits, padding, scale in ((64, False, 1.0), (32, True, -2.7)):
+        table, index, _ = _case(n, rows, width, dtype, cuda, bits=bits, padding=padding)
+        got = embedding.lookup(table, index, scale=scale, padding_index=-1 if padding else None,
+                               p=p, seed=SEED, offset=OFFSET)
+        assert got.dtype == dtype and got.shape == (n, width)
+        _check_lookup(got, table, index, scale, p, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,rows,width", SIZES)
+@pytest.mark.parametrize("p", [0.0, 0.3])
+def test_gradient(cuda, dtype, n, rows, width, p):
+    import embedding
+
+    for kind, bits, padding, scale in (("uniform", 64, False, 1.0), ("skewed", 32, True, 0.3),
+                                       ("same", 64, True, 1.0)):
+        _, index, grad = _case(n, rows, width, dtype, cuda, kind=kind, bits=bits, padding=padding)
+        got = embedding.lookup_gradient(grad, index, rows, scale=scale, p=p, seed=SEED,
+                                        padding_index=-1 if padding else None, offset=OFFSET)
+        assert got.dtype == dtype
+        _check_gradient(got, grad, index, rows, scale, p, dtype)
+
+
+@pytest.mark.parametrize("kind", ["uniform", "skewed", "same", "sorted", "distinct"])
+@pytest.mark.parametrize("n,rows", [(1, 1), (100, 1000), (4096, 255), (4097, 256), (8191, 1023),
+                                    (8193, 1024), (50_000, 70_000), (300_001, 4096),
+                                    (65_537, 3_000_000)])
+def test_order(cuda, kind, n, rows):
+    """The stable order, tokens without a row last."""
+    import embedding
+
+    for bits, padding in ((64, False), (32, True)):
+        _, index, _ = _case(n, rows, 1, torch.float32, cuda, kind=kind, bits=bits, padding=padding)
+        order = embedding.token_order(index, rows, padding_index=-1 if padding else None)
+        i = index.cpu().numpy().astype(np.int64)
+        i = np.where(i < 0, rows, i)
+        place = np.argsort(i, kind="stable")
+        assert np.array_equal(order.pairs.cpu().numpy(), np.stack([i[place], place], axis=1))
+
+
+@pytest.mark.parametrize("kind", ["skewed", "same", "distinct"])
+@pytest.mark.parametrize("n,rows,width", [(100_003, 4096, 48), (65_000, 60_000, 20),
+                                          (300_000, 17, 5), (9000, 3, 513)])
+def test_long_and_wide_sums(cuda, kind, n, rows, width):
+    """Rows whose tokens lie in very many chunks; given and made orders agree
+    bit for bit, and so do two runs."""
+    import embedding
+
+    _, index, grad = _case(n, rows, width, torch.float32, cuda, kind=kind)
+    got = embedding.lookup_gradient(grad, index, rows)
+    _check_gradient(got, grad, index, rows, 1.0, 0.0, torch.float32)
+    order = embedding.token_order(index, rows)
+    assert torch.equal(got, embedding.lookup_gradient(grad, None, rows, order=order))
+    assert torch.equal(got, embedding.lookup_gradient(grad, index, rows))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_layouts(cuda, dtype):
+    """Strided and unaligned tables and gradients, indices of any shape, expanded
+    and transposed gradients."""
+    import embedding
+
+    n, rows = 300, 50
+    for width, gap, skip in ((48, 16, 0), (48, 5, 0), (48, 8, 1), (9, 3, 2), (64, 0, 0), (2, 6, 2)):
+        table, index, grad = _case(n, rows, width + gap, dtype, cuda)
+        table, grad = table[:, skip:skip + width], grad[:, skip:skip + width]
+        got = embedding.lookup(table, index.view(3, 4, 25), p=0.2, seed=SEED, offset=OFFSET)
+        assert got.shape == (3, 4, 25, width) and got.is_contiguous()
+        _check_lookup(got, table, index, 1.0, 0.2, dtype)
+        got = embedding.lookup_gradient(grad, index.view(20, 15), rows, p=0.2, seed=SEED,
+                                        offset=OFFSET)
+        _check_gradient(got, grad, index, rows, 1.0, 0.2, dtype)
+    wide = torch.stack([index, index], dim=1)[:, 0]  # strided indices
+    assert torch.equal(embedding.lookup(table, wide), embedding.lookup(table, index))
+    for g in (grad[:1].expand(n, 2), grad.t().contiguous().t(), grad[0, :1].expand(n, 2),
+              grad.reshape(20, 15, 2).transpose(0, 1)):
+        i = index if g.dim() == 2 else index.view(20, 15).t()
+        _check_gradient(embedding.lookup_gradient(g, i, rows), g.reshape(n, 2), i, rows, 1.0,
+                        0.0, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_nothing_to_do(cuda, dtype):
+    import embedding
+
+    none = torch.empty(0, dtype=torch.int64, device=cuda)
+    table = torch.ones(4, 3, dtype=dtype, device=cuda)
+    assert embedding.lookup(table, none).shape == (0, 3)
+    got = embedding.lookup_gradient(torch.empty(0, 3, dtype=dtype, device=cuda), none, 4)
+    assert got.shape == (4, 3) and not got.any()
+    assert embedding.token_order(none, 4).pairs.shape == (0, 2)
+    only_padding = torch.full((70,), 9, device=cuda)
+    assert not embedding.lookup(table, only_padding, padding_index=9).any()
+    g = torch.full((70, 3), float("nan"), dtype=dtype, device=cuda)
+    assert not embedding.lookup_gradient(g, only_padding, 4, padding_index=9).any()
+    one = torch.zeros(5, dtype=torch.int32, device=cuda)
+    assert embedding.lookup(torch.ones(4, 0, dtype=dtype, device=cuda), one).shape == (5, 0)
+    assert embedding.lookup_gradient(torch.ones(5, 0, dtype=dtype, device=cuda), one, 4).shape == (4, 0)
+    # A padding index inside the table: its row is neither read nor given anything.
+    index = torch.tensor([0, 1, 2, 1], device=cuda)
+    table = torch.arange(12, device=cuda).view(4, 3).to(dtype) + 1
+    assert embedding.lookup(table, index, padding_index=1)[[1, 3]].eq(0).all()
+    assert embedding.lookup_gradient(torch.ones(4, 3, dtype=dtype, device=cuda), index, 4,
+                                     padding_index=1).tolist() == [[1] * 3, [0] * 3, [1] * 3, [0] * 3]
+    # Everything dropped.
+    assert not embedding.lookup(table, index, p=1.0).any()
+    assert not embedding.lookup_gradient(torch.ones(4, 3, dtype=dtype, device=cuda), index, 4,
+                                         p=1).any()
+
+
+def test_indices_outside_the_table(cuda):
+    """They read nothing, give nothing and set the fault word."""
+    import _native as native
+    import embedding
+
+    native.fault_status()
+    table = torch.ones(4, 8, device=cuda)
+    for bits in (torch.int64, torch.int32):
+        bad = torch.tensor([0, 4, -1, 2 ** 31 - 1, -2 ** 31, 3], device=cuda).to(bits)
+        got = embedding.lookup(table, bad)
+        assert got.sum(1).tolist() == [8, 0, 0, 0, 0, 8]
+        assert native.fault_status() == 256 and native.fault_status() == 0
+        got = embedding.lookup_gradient(torch.ones(6, 8, device=cuda), bad, 4)
+        assert got.sum(1).tolist() == [8, 0, 0, 8]
+        assert native.fault_status() == 256
+    far = torch.tensor([2 ** 32, 2 ** 62, -2 ** 63, 1], device=cuda)
+    assert embedding.lookup(table, far).sum(1).tolist() == [0, 0, 0, 8]
+    assert native.fault_status() == 256
+    assert embedding.lookup(table, far, padding_index=2 ** 32)[3].tolist() == [1] * 8
+    assert native.fault_status() == 256
+    embedding.lookup(table, torch.tensor([-7, 1], device=cuda), padding_index=-7)
+    assert native.fault_status() == 0
+
+
+def test_infinities_and_nan_stay_where_they_are(cuda):
+    import embedding
+
+    index = torch.tensor([0, 1, 1, 2, 0], device=cuda)
+    grad = torch.ones(5, 4, device=cuda)
+    grad[1, 0], grad[2, 1], grad[3, 2] = float("inf"), float("nan"), -float("inf")
+    got = embedding.lookup_gradient(grad, index, 4)
+    assert got[0].tolist() == [2] * 4 and got[3].tolist() == [0] * 4
+    assert got[1, 0] == float("inf") and torch.isnan(got[1, 1]) and got[1, 2:].tolist() == [2, 2]
+    assert got[2, 2] == -float("inf") and got[2, [0, 1, 3]].tolist() == [1] * 3
+    # Dropped, they are gone.
+    grad = torch.full((64, 16), float("nan"), device=cuda)
+    kept = draws.keep(np.arange(1024), 0.5, 3, 4).reshape(64, 16)
+    got = embedding.lookup_gradient(grad, torch.arange(64, device=cuda), 64, p=0.5, seed=3, offset=4)
+    assert np.array_equal(torch.isnan(got).cpu().numpy(), kept) and not got.nan_to_num().any()
+
+
+def test_far_rows(cuda):
+    """Element offsets past 2^32 in the table and in its gradient."""
+    import embedding
+
+    rows, width = 66_000, 65_600
+    table = torch.zeros(rows, width, dtype=torch.float16, device=cuda)
+    table[rows - 1] = 3.0
+    table[65_536] = 2.0
+    index = torch.tensor([rows - 1, 0, 65_536], device=cuda)
+    assert embedding.lookup(table, index)[:, [0, width - 1]].tolist() == [[3, 3], [0, 0], [2, 2]]
+    del table
+    grad = torch.arange(1, 4, device=cuda).to(torch.float16).view(3, 1).expand(3, width)
+    got = embedding.lookup_gradient(grad, index, rows)
+    assert got[index][:, [0, 1, width - 1]].tolist() == [[1] * 3, [2] * 3, [3] * 3]
+    assert [int(got[r].any()) for r in (1, 65_535, 65_537, rows - 2)] == [0] * 4
+
+
+# ---------------------------------------------------------------------------
+# Adam.
+
+def _adam_state(rows, width, cuda, seed=5):
+    g = torch.Generator(device="cpu").manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g)
+    return [t.to(cuda) for t in (r(rows, width) * 0.05, r(rows, width) * 1e-3,
+                                 torch.rand(rows, width, generator=g) * 3e-6 + 1e-6)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,rows,width,p", [(1, 3, 5, 0.0), (500, 70, 48, 0.0), (500, 2000, 45, 0.4),
+                                            (5000, 3, 130, 0.2), (0, 4, 6, 0.0)])
+def test_consume_against_64_bits(cuda, dtype, n, rows, width, p):
+    import embedding
+
+    step, rate = 20, 0.0025
+    b1, b2 = 1 - 0.9 ** step, math.sqrt(1 - 0.999 ** step)
+    _, index, grad = _case(n, rows, width, dtype, cuda, kind="skewed", padding=n > 1)
+    grad = grad * 1e-3
+    state = _adam_state(rows, width, cuda)
+    t, m, v = [x.double().cpu().numpy() for x in state]
+    embedding.consume_torch_adam(*state, grad, index, rate=rate, bias1=b1, bias2_sqrt=b2,
+                                 scale=0.7, padding_index=-1, p=p, seed=SEED, offset=OFFSET)
+    g, i = grad.double().cpu().numpy() * 0.7, index.cpu().numpy()
+    if p > 0:
+        g = g * draws.weight(g.shape, p, SEED, OFFSET)
+    total, size = np.zeros((rows, width)), np.zeros((rows, width))
+    np.add.at(total, i[i >= 0], g[i >= 0])
+    np.add.at(size, i[i >= 0], np.abs(g[i >= 0]))
+    off = size * (np.bincount(i[i >= 0], minlength=rows)[:, None] + 2.01) * U  # of the gradient
+    m1, v1 = 0.9 * m + 0.1 * total, 0.999 * v + 0.001 * total ** 2
+    move = rate / b1 / (np.sqrt(v1) / b2 + 1e-15)
+    # Moments: the gradient's error through the formula, one rounding each.
+    off_m = 0.1 * off + 1.01 * U * np.abs(m1)
+    off_v = 0.001 * (2 * np.abs(total) + off) * off + 1.01 * U * v1
+    # The step: those, and at most eight roundings of its own (rate / bias1 and
+    # the bias correction to float, root, ratio, product, quotient).
+    off_t = move * (off_m + (np.abs(m1) + off_m) * (off_v / v1 + 8 * U)) + 1.01 * U * np.abs(t)
+    for got, want, limit in zip(state, (t - move * m1, m1, v1), (off_t, off_m, off_v)):
+        assert (np.abs(got.double().cpu().numpy() - want) <= limit).all()
+
+
+def _fused_adam(p, m, v, g, rate, b1, b2):
+    """The framework's torch-fused Adam, operation by operation: moments in double
+    rounded to float, step size rate / bias1 in float, eps added in double."""
+    f, d = np.float32, np.float64
+    g = g.astype(d)
+    m = (d(0.9) * m.astype(d) + (d(1) - d(0.9)) * g).astype(f)
+    v = (d(0.999) * v.astype(d) + ((d(1) - d(0.999)) * g) * g).astype(f)
+    denom = ((np.sqrt(v) / f(b2)).astype(d) + d(1e-15)).astype(f)
+    return p - (f(rate / d(f(b1))) * m) / denom, m, v
+
+
+@pytest.mark.parametrize("n,rows,width", [(900, 50, 48), (70, 300, 7), (20_000, 11, 64)])
+def test_consume_is_the_frameworks_adam(cuda, n, rows, width):
+    """Three steps agree bit for bit with the restated Adam on the gradient that
+    lookup_gradient writes."""
+    import embedding
+
+    table = _adam_state(rows, width, cuda)[0]
+    first, second = torch.zeros_like(table), torch.zeros_like(table)
+    want = [t.cpu().numpy() for t in (table, first, second)]
+    for step in (1, 2, 3):
+        _, index, grad = _case(n, rows, width, torch.float32, cuda, kind="skewed", seed=step)
+        g = embedding.lookup_gradient(grad, index, rows, scale=0.3)
+        b1 = float(np.float32(1 - 0.9 ** step))
+        b2 = float(np.float32(math.sqrt(1 - 0.999 ** step)))
+        want = _fused_adam(*want, g.cpu().numpy(), 0.0025, b1, b2)
+        embedding.consume_torch_adam(table, first, second, grad, index, rate=0.0025, bias1=b1,
+                                     bias2_sqrt=b2, scale=0.3)
+        for got, value in zip((table, first, second), want):
+            assert np.array_equal(got.cpu().numpy(), value)
+
+
+# ---------------------------------------------------------------------------
+# Autograd, graphs, streams, refusals.
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_autograd(cuda, dtype):
+    import embedding
+
+    table, index, grad = _case(700, 90, 48, dtype, cuda, kind="skewed")
+    table.requires_grad_(True)
+    order = embedding.token_order(index, 90)
+    for given in (None, order):
+        y = embedding.lookup(table, index, scale=1.5, p=0.2, seed=SEED, offset=OFFSET, order=given)
+        (got,) = torch.autograd.grad(y, table, grad)
+        _check_gradient(got, grad, index, 90, 1.5, 0.2, dtype)
+    (got,) = torch.autograd.grad(embedding.lookup(table, index).sum(), table)
+    _check_gradient(got, torch.ones_like(grad), index, 90, 1.0, 0.0, dtype)
+    y = embedding.lookup(table, index)
+    with pytest.raises(RuntimeError, match="first-order"):
+        torch.autograd.grad(y.sum(), table, create_graph=True)
+    index.add_(0)  # written after the forward pass
+    with pytest.raises(RuntimeError):
+        y.sum().backward()
+
+
+def test_gradient_against_differences(cuda):
+    """The lookup is linear, so a difference quotient of small integers and
+    powers of two is the derivative exactly."""
+    import embedding
+
+    index = torch.tensor([0, 2, 2, 1, 2], device=cuda)
+    weight = torch.arange(1, 21, device=cuda).float().view(5, 4)
+    table = torch.ones(4, 4, device=cuda, requires_grad=True)
+    value = lambda t: (embedding.lookup(t, index, scale=2.0, p=0.5, seed=1, offset=2) * weight).sum()
+    (got,) = torch.autograd.grad(value(table), table)
+    with torch.no_grad():
+        for k in range(4):
+            for d in range(4):
+                moved = table.detach().clone()
+                moved[k, d] += 0.5
+                assert (value(moved) - value(table)).item() / 0.5 == got[k, d].item()
+
+
+def test_fused_dropout_is_the_dropout(cuda):
+    """Lookup with p is dropout of the lookup (factors whose product is exact)."""
+    import dropout
+    import embedding
+
+    table, index, _ = _case(999, 50, 77, torch.float32, cuda)
+    got = embedding.lookup(table, index, scale=2.0, p=0.5, seed=SEED, offset=OFFSET)
+    want = dropout.dropout(embedding.lookup(table, index, scale=2.0), 0.5, SEED, OFFSET)
+    assert torch.equal(got, want)
+
+
+def test_training_step_under_a_graph(cuda):
+    """Lookup, dropout and backward captured twice; replays follow new indices and
+    a new offset."""
+    import embedding
+
+    rows, width, n = 60, 48, 5000
+    table, index, grad = _case(n, rows, width, torch.float32, cuda, kind="skewed")
+    table.requires_grad_(True)
+    offset = torch.zeros(1, dtype=torch.int64, device=cuda)
+
+    def step():
+        y = embedding.lookup(table, index, p=0.25, seed=SEED, offset=offset)
+        return y.detach(), torch.autograd.grad(y, table, grad)[0]
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    first, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(first):
+        a = step()
+    with torch.cuda.graph(second):
+        b = step()
+    for seed in (1, 2):
+        index.copy_(_case(n, rows, width, torch.float32, cuda, kind="skewed", seed=seed)[1])
+        offset.fill_(seed * 2 ** 33)
+        first.replay()
+        second.replay()
+        for y, g in (a, b):
+            _check_lookup(y, table.detach(), index, 1.0, 0.25, torch.float32, seed * 2 ** 33)
+            _check_gradient(g, grad, index, rows, 1.0, 0.25, torch.float32, seed * 2 ** 33)
+
+
+def test_two_streams_at_once(cuda):
+    import embedding
+
+    cases = [_case(20_000, 500, 48, torch.float32, cuda, kind="skewed", seed=s) for s in (0, 1)]
+    want = [embedding.lookup_gradient(g, i, 500) for _, i, g in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(5):
+        got = []
+        for stream, (_, i, g) in zip(streams, cases):
+            with torch.cuda.stream(stream):
+                got.append(embedding.lookup_gradient(g, i, 500))
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+def test_refusals(cuda):
+    import embedding
+
+    table, index, grad = _case(10, 4, 6, torch.float32, cuda)
+    state = _adam_state(4, 6, cuda)
+    order = embedding.token_order(index, 4)
+    adam = dict(rate=0.1, bias1=0.5, bias2_sqrt=0.5)
+    calls = [
+        lambda: embedding.lookup(table.double(), index),
+        lambda: embedding.lookup(table.view(2, 2, 6), index),
+        lambda: embedding.lookup(table, index.float()),
+        lambda: embedding.lookup(table, index.cpu()),
+        lambda: embedding.lookup(table, index, scale=float("inf")),
+        lambda: embedding.lookup(table, index, p=-1.0),
+        lambda: embedding.lookup(table, index, padding_index=1.5),
+        lambda: embedding.lookup_gradient(grad, index[:9], 4),
+        lambda: embedding.lookup_gradient(grad, index, -1),
+        lambda: embedding.lookup_gradient(grad, None, 5, order=order),
+        lambda: embedding.lookup_gradient(grad[:9], None, 4, order=order),
+        lambda: embedding.lookup_gradient(grad.double(), index, 4),
+        lambda: embedding.lookup_gradient(grad, index, 4, seed=-1),
+        lambda: embedding.consume_torch_adam(*state, grad[:, :5], index, **adam),
+        lambda: embedding.consume_torch_adam(state[0], state[1], state[1], grad, index, **adam),
+        lambda: embedding.consume_torch_adam(*state[:2], state[2].half(), grad, index, **adam),
+        lambda: embedding.consume_torch_adam(*state, grad, index, **{**adam, "bias1": 0.0}),
+        lambda: embedding.consume_torch_adam(*state, grad, index, **{**adam, "rate": float("nan")}),
+        lambda: embedding.lookup(table.requires_grad_(True), index[:5], order=order),
+    ]
+    before = [t.clone() for t in state]
+    for call in calls:
+        with pytest.raises(RuntimeError):
+            call()
+    assert all(torch.equal(a, b) for a, b in zip(state, before))
+
+
+def test_lookup_feeds_the_renderer(cuda):
+    """Codebook colours as they would be used: lookup, render, backward through
+    the renderer, Adam on the codebook; the same numbers as the step with the
+    gathered coefficients as leaves."""
+    import embedding
+    from data_parallel import orbit_camera
+    from rasterizer import GaussianRasterizationSettings, GaussianRasterizer
+
+    n, codes = 3000, 40
+    rng = np.random.default_rng(3)
+    f = lambda a: torch.from_numpy(np.asarray(a, np.float32)).to(cuda)
+    means = f(rng.uniform(-1, 1, (n, 3)))
+    scales, rotations = f(np.full((n, 3), 0.03)), f(rng.standard_normal((n, 4)))
+    rotations = rotations / rotations.norm(dim=1, keepdim=True)
+    opacity = f(rng.uniform(0.2, 0.9, (n, 1)))
+    camera = orbit_camera(1, 8, width=160, height=120, device=cuda)
+    settings = GaussianRasterizationSettings(
+        120, 160, camera.tan_x, camera.tan_y, torch.zeros(3, device=cuda), 1.0, camera.view,
+        camera.proj, 3, camera.campos, False, False)
+    index = torch.from_numpy(rng.integers(0, codes, n)).to(cuda)
+    codebook = f(rng.normal(0.0, 0.2, (codes, 48))).requires_grad_(True)
+    leaf = codebook.detach()[index].view(n, 16, 3).requires_grad_(True)
+    weight = f(rng.standard_normal((3, 120, 160)))
+
+    def image(sh):
+        return GaussianRasterizer(settings)(means, torch.zeros_like(means), opacity, shs=sh,
+                                            scales=scales, rotations=rotations)[0]
+
+    got = image(embedding.lookup(codebook, index).view(n, 16, 3))
+    want = image(leaf)
+    assert torch.equal(got, want) and got.abs().sum() > 0
+    (g,) = torch.autograd.grad((got * weight).sum(), codebook)
+    (h,) = torch.autograd.grad((want * weight).sum(), leaf)
+    # The renderer's atomics add in any order: the per-Gaussian adjoints of two
+    # runs agree to about n roundings of their size, far below this limit.
+    size = torch.zeros_like(g).index_add_(0, index, h.view(n, 48).abs())
+    total = torch.zeros_like(g).index_add_(0, index, h.view(n, 48))
+    assert (g - total).abs().le(1e-4 * size + 1e-12).all() and g.abs().sum() > 0
+    first, second = torch.zeros_like(g), torch.zeros_like(g)
+    before = codebook.detach().clone()
+    with torch.no_grad():
+        embedding.consume_torch_adam(codebook, first, second, h.view(n, 48), index, rate=0.0025,
+                                     bias1=0.1, bias2_sqrt=math.sqrt(0.001))
+    assert (codebook.detach() - before).abs().max() <= 0.0026 and (first != 0).any()
