@@ -65,4 +65,16 @@ __device__ __forceinline__ uint32_t word_of(const uint4& w, unsigned j) {
   return j == 0 ? w.x : j == 1 ? w.y : j == 2 ? w.z : w.w;
 }
 
+// The decisions for V elements that begin at element e.
+template <int V>
+__device__ __forceinline__ void mask_vector(const CounterMask& m, unsigned long long offset,
+                                            int64_t e, bool (&keep)[V]) {
+  uint4 words = mask_words(m, offset, e / 4);
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    if (j > 0 && (e + j) % 4 == 0) words = mask_words(m, offset, (e + j) / 4);
+    keep[j] = m.keeps(word_of(words, unsigned(e + j) % 4));
+  }
+}
+
 }  // namespace clad3dgs
