@@ -43,80 +43,149 @@ using tokens::Index;
 
 constexpr int kThreads = 256;
 
-// How a row is cut: vectors of V elements, `lanes` of them side by side in one
-// group (a power of two, 32 at most), `slices` groups a row.
-struct Cut {
-  int lanes;
-  int64_t slices;
-};
-
-Cut cut_of(int64_t width, int vec) {
-  const int64_t vectors = width / vec;
-  Cut c{1, 0};
-  while (c.lanes < 32 && c.lanes < vectors) c.lanes *= 2;
-  c.slices = (vectors + c.lanes - 1) / c.lanes;
-  return c;
-}
-
-template <class T, int V, bool kDrop>
+// A lookup moves rows through registers: bound by writing the output, the index
+// and the table's rows (small ones stay in L2) come on top. Groups of lanes take
+// a row each, C vectors of 16 bytes a lane; a thread asks for the rows of U
+// tokens before it stores the first, so that four to six loads are in flight.
+template <class T, int V, int C, int U, bool kDrop>
 __global__ void __launch_bounds__(kThreads)
-    lookup_kernel(int64_t n, int64_t width, Cut cut, const T* __restrict__ table,
-                  int64_t table_stride, Index index, float factor, CounterMask mask,
-                  T* __restrict__ out) {
+    lookup_kernel(int64_t n, int64_t width, int lanes, int64_t slices,
+                  const T* __restrict__ table, int64_t table_stride, Index index, float factor,
+                  CounterMask mask, T* __restrict__ out) {
   const unsigned long long offset = kDrop ? mask_offset(mask) : 0;
-  const int lane = threadIdx.x % cut.lanes;
-  const int64_t groups = int64_t(gridDim.x) * kThreads / cut.lanes;
-  for (int64_t job = (blockIdx.x * int64_t(kThreads) + threadIdx.x) / cut.lanes;
-       job < n * cut.slices; job += groups) {
-    const int64_t i = job / cut.slices;
-    const int64_t column = ((job - i * cut.slices) * cut.lanes + lane) * V;
-    if (column >= width) continue;
-    const uint32_t row = tokens::row_of(index, i);
-    Vec<T, V> v{};
-    if (row < index.rows) {
-      v = *reinterpret_cast<const Vec<T, V>*>(table + row * table_stride + column);
+  const int64_t block = blockIdx.x / slices;
+  const int lane = threadIdx.x % lanes, groups = kThreads / lanes;
+  const int apart = lanes * V;
+  const int64_t column = (blockIdx.x - block * slices) * (apart * C) + lane * V;
+  const int64_t first = block * (groups * U) + threadIdx.x / lanes;
+  int64_t raw[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    raw[u] = first + u * groups < n ? tokens::raw_index(index, first + u * groups) : 0;
+  Vec<T, V> v[U][C];
+  uint32_t row[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    row[u] = first + u * groups < n ? tokens::row_of(index, raw[u]) : uint32_t(index.rows);
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      v[u][c] = {};
+      if (row[u] < index.rows && column + c * apart < width)
+        v[u][c] = *reinterpret_cast<const Vec<T, V>*>(table + row[u] * table_stride + column +
+                                                      c * apart);
+    }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t i = first + u * groups;
+    if (i >= n) return;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int64_t at = i * width + column + c * apart;
+      if (column + c * apart >= width) break;
       bool keep[V];
-      if (kDrop) mask_vector<V>(mask, offset, i * width + column, keep);
+      if (kDrop) mask_vector<V>(mask, offset, at, keep);
 #pragma unroll
       for (int j = 0; j < V; ++j)
-        v.v[j] = from_float<T>(!kDrop || keep[j] ? to_float(v.v[j]) * factor : 0.f);
+        v[u][c].v[j] = from_float<T>(!kDrop || keep[j] ? to_float(v[u][c].v[j]) * factor : 0.f);
+      if (row[u] >= index.rows) v[u][c] = {};
+      *reinterpret_cast<Vec<T, V>*>(out + at) = v[u][c];
     }
-    *reinterpret_cast<Vec<T, V>*>(out + i * width + column) = v;
   }
 }
 
-template <class T, int V>
-cudaError_t run_lookup(int64_t n, int64_t width, const void* table, int64_t stride,
-                       const Index& index, float factor, const CounterMask& mask, bool drop,
-                       void* out, cudaStream_t stream) {
-  const Cut cut = cut_of(width, V);
-  const int64_t threads = n * cut.slices * cut.lanes;
-  const unsigned grid =
-      unsigned(std::min<int64_t>((threads + kThreads - 1) / kThreads, int64_t(1) << 20));
-  auto* kernel = drop ? lookup_kernel<T, V, true> : lookup_kernel<T, V, false>;
-  kernel<<<grid, kThreads, 0, stream>>>(n, width, cut, static_cast<const T*>(table), stride,
-                                        index, factor, mask, static_cast<T*>(out));
+// Rows that do not start on 16 bytes: a thread fills V consecutive elements of
+// the output, whatever rows they belong to, from single loads (adjacent
+// threads read adjacent elements, which the L1 cache gathers).
+template <class T, class Number, int V, bool kDrop>
+__global__ void __launch_bounds__(kThreads)
+    lookup_flat_kernel(Number total, Number width, const T* __restrict__ table,
+                       int64_t table_stride, Index index, float factor, CounterMask mask,
+                       T* __restrict__ out) {
+  const unsigned long long offset = kDrop ? mask_offset(mask) : 0;
+  const Number at = (Number(blockIdx.x) * kThreads + threadIdx.x) * V;
+  if (at >= total) return;
+  Number i = at / width, column = at - i * width;
+  uint32_t row = tokens::row_of(index, tokens::raw_index(index, i));
+  Vec<T, V> v{};
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    if (at + j < total) {
+      if (column == width) {
+        column = 0;
+        row = tokens::row_of(index, tokens::raw_index(index, ++i));
+      }
+      if (row < index.rows) v.v[j] = table[row * table_stride + column];
+      ++column;
+    }
+  }
+  bool keep[V];
+  if (kDrop) mask_vector<V>(mask, offset, at, keep);
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+    v.v[j] = from_float<T>(!kDrop || keep[j] ? to_float(v.v[j]) * factor : 0.f);
+  if (at + V <= total) {
+    *reinterpret_cast<Vec<T, V>*>(out + at) = v;
+  } else {
+    for (int j = 0; j < V; ++j)
+      if (at + j < total) out[at + j] = v.v[j];
+  }
+}
+
+struct Lookup {
+  int64_t n, width;
+  const void* table;
+  int64_t stride;
+  Index index;
+  float factor;
+  CounterMask mask;
+  bool drop;
+  void* out;
+  cudaStream_t stream;
+};
+
+template <class T, int V, int C, int U>
+cudaError_t run_rows(const Lookup& a) {
+  int64_t padded;
+  const int lanes = sums::lanes_of(a.width / V, C, &padded);
+  const int64_t slices = padded / (lanes * C), tokens = kThreads / lanes * U;
+  const unsigned grid = unsigned((a.n + tokens - 1) / tokens * slices);
+  auto* kernel = a.drop ? lookup_kernel<T, V, C, U, true> : lookup_kernel<T, V, C, U, false>;
+  kernel<<<grid, kThreads, 0, a.stream>>>(a.n, a.width, lanes, slices,
+                                          static_cast<const T*>(a.table), a.stride, a.index,
+                                          a.factor, a.mask, static_cast<T*>(a.out));
+  return cudaGetLastError();
+}
+
+template <class T, class Number, int V>
+cudaError_t run_flat(const Lookup& a) {
+  const int64_t total = a.n * a.width;
+  const unsigned grid = unsigned((total + kThreads * V - 1) / (kThreads * V));
+  auto* kernel =
+      a.drop ? lookup_flat_kernel<T, Number, V, true> : lookup_flat_kernel<T, Number, V, false>;
+  kernel<<<grid, kThreads, 0, a.stream>>>(Number(total), Number(a.width),
+                                          static_cast<const T*>(a.table), a.stride, a.index,
+                                          a.factor, a.mask, static_cast<T*>(a.out));
   return cudaGetLastError();
 }
 
 template <class T>
-cudaError_t pick_lookup(int64_t n, int64_t width, const void* table, int64_t stride,
-                        const Index& index, float factor, const CounterMask& mask, bool drop,
-                        void* out, cudaStream_t stream) {
-  const int bytes = common_bytes(uint64_t(width * sizeof(T)) | uint64_t(stride * sizeof(T)) |
-                                 uint64_t(table) | uint64_t(out));
-  auto go = [&](auto run) {
-    return run(n, width, table, stride, index, factor, mask, drop, out, stream);
-  };
-  if constexpr (sizeof(T) == 2) {
-    if (bytes >= 16) return go(run_lookup<T, 8>);
-    if (bytes >= 8) return go(run_lookup<T, 4>);
-    if (bytes >= 4) return go(run_lookup<T, 2>);
-  } else {
-    if (bytes >= 16) return go(run_lookup<T, 4>);
-    if (bytes >= 8) return go(run_lookup<T, 2>);
+cudaError_t run_lookup(const Lookup& a) {
+  constexpr int V = 16 / sizeof(T);
+  const int bytes = common_bytes(uint64_t(a.width * sizeof(T)) | uint64_t(a.stride * sizeof(T)) |
+                                 uint64_t(a.table) | uint64_t(a.out));
+  if (bytes >= 16) {
+    switch (sums::vectors_of_lane(a.n, a.width, V)) {
+      case 4: return run_rows<T, V, 4, 1>(a);
+      case 3: return run_rows<T, V, 3, 2>(a);
+      default: return run_rows<T, V, 1, 4>(a);
+    }
   }
-  return go(run_lookup<T, 1>);
+  if (uint64_t(a.out) % 16) return run_flat<T, int64_t, 1>(a);
+  // Divisions of 32-bit numbers while every element number fits one.
+  return a.n * a.width < (int64_t(1) << 32) - kThreads * V ? run_flat<T, uint32_t, V>(a)
+                                                           : run_flat<T, int64_t, V>(a);
 }
 
 int refuse(const char* what, const char* why) {
@@ -190,11 +259,11 @@ extern "C" int clad3dgs_token_order(int64_t n, int64_t rows, const void* index, 
   if (const char* why = problem(n, rows, 0, CLAD3DGS_F32, 1.0, 0.0)) return refuse(what, why);
   if (index_bits != 32 && index_bits != 64) return refuse(what, "indices are 32 or 64 bits");
   if (n == 0) return CLAD3DGS_OK;
-  if (!index || !order || !workspace) return refuse(what, "null array");
+  const size_t need = tokens::sort_plan(n, rows).bytes();
+  if (!index || !order || (need > 0 && !workspace)) return refuse(what, "null array");
   if (uint64_t(workspace) % 256 || uint64_t(order) % 8)
     return refuse(what, "unaligned workspace or order");
-  if (workspace_bytes < tokens::sort_plan(n, rows).bytes())
-    return refuse(what, "workspace too small");
+  if (workspace_bytes < need) return refuse(what, "workspace too small");
   const tokens::Index x{index, index_bits == 64, has_padding != 0, padding, rows};
   return status(what, tokens::sort_tokens(n, x, reinterpret_cast<uint2*>(order), workspace,
                                           stream));
@@ -213,15 +282,12 @@ extern "C" int clad3dgs_embedding_lookup(int type, int64_t n, int64_t rows, int6
   if ((!table && rows > 0) || !index || !out) return refuse(what, "null array");
   if (table_stride < 0) return refuse(what, "bad row stride");
   const tokens::Index x{index, index_bits == 64, has_padding != 0, padding, rows};
-  const CounterMask mask =
-      counter_mask(p, seed, offset, reinterpret_cast<const long long*>(offset_device));
-  auto go = [&](auto pick) {
-    return pick(n, width, table, table_stride, x, factor_of(scale, p), mask, p > 0.0, out,
-                stream);
-  };
-  return status(what, type == CLAD3DGS_F32   ? go(pick_lookup<float>)
-                      : type == CLAD3DGS_F16 ? go(pick_lookup<__half>)
-                                             : go(pick_lookup<__nv_bfloat16>));
+  const Lookup a{n, width, table, table_stride, x, factor_of(scale, p),
+                 counter_mask(p, seed, offset, reinterpret_cast<const long long*>(offset_device)),
+                 p > 0.0, out, stream};
+  return status(what, type == CLAD3DGS_F32   ? run_lookup<float>(a)
+                      : type == CLAD3DGS_F16 ? run_lookup<__half>(a)
+                                             : run_lookup<__nv_bfloat16>(a));
 }
 
 extern "C" size_t clad3dgs_embedding_workspace(int64_t n, int64_t width) {

@@ -3,15 +3,19 @@
 // (padding, or an index outside the table) get the row number `rows` and so
 // come last.
 //
-// Least-significant-digit radix sort, at most ten bits a pass. A pass is three
-// kernels: every block counts the digits of its tile; one warp per digit turns
-// the blocks' counts into exclusive sums; every block ranks its tile and
-// scatters it. Ranks come from ballots of equal digits within a warp, taken in
-// token order, so the sort is stable and the order the same on every run.
+// Least-significant-digit radix sort. Ranks come from the lanes of a warp that
+// hold equal digits, in token order, so the sort is stable and the order the
+// same on every run.
+//
+// Up to kSmall tokens: one block sorts in shared memory, all passes in one
+// launch. More: two kernels a pass; every block (one an SM at most) counts the
+// digits of a contiguous share of the tokens, then adds up the other blocks'
+// counts itself (they lie in L2) and scatters its share tile by tile. Bound by
+// latency at these sizes: everything a thread reads of a tile is asked for
+// before any of it is used.
 #pragma once
 #include <cuda_runtime.h>
 
-#include <algorithm>
 #include <cstdint>
 
 namespace clad3dgs {
@@ -30,184 +34,339 @@ struct Index {
   int64_t rows;
 };
 
-// The row that token i names, or `rows` for none.
-__device__ __forceinline__ uint32_t row_of(const Index& x, int64_t i) {
-  const int64_t t = x.wide ? static_cast<const int64_t*>(x.data)[i]
-                           : int64_t(static_cast<const int32_t*>(x.data)[i]);
-  if (x.has_padding && t == x.padding) return uint32_t(x.rows);
-  if (t >= 0 && t < x.rows) return uint32_t(t);
-  atomicOr(&g_token_fault, kFaultTokenRange);
+__device__ __forceinline__ int64_t raw_index(const Index& x, int64_t i) {
+  return x.wide ? static_cast<const int64_t*>(x.data)[i]
+                : int64_t(static_cast<const int32_t*>(x.data)[i]);
+}
+
+// The row that an index names, or `rows` for none. (Apart from the load: a
+// thread loads all its indices before the first of these, whose atomic would
+// hold the later loads back.)
+__device__ __forceinline__ uint32_t row_of(const Index& x, int64_t t) {
+  if (t >= 0 && t < x.rows && !(x.has_padding && t == x.padding)) return uint32_t(t);
+  if (!(x.has_padding && t == x.padding)) atomicOr(&g_token_fault, kFaultTokenRange);
   return uint32_t(x.rows);
 }
 
-constexpr int kSortThreads = 256;
-constexpr int kSortWarps = kSortThreads / 32;
-constexpr int kSortItems = 16;
-constexpr int kSortTile = kSortThreads * kSortItems;
-constexpr int kDigitBits = 10;
-
-struct SortPlan {
-  int passes, bits;  // digit width of every pass
-  int64_t blocks;
-  size_t pair_bytes, count_bytes, total_bytes;  // workspace parts
-
-  size_t bytes() const { return pair_bytes + count_bytes + total_bytes; }
-};
-
-inline SortPlan sort_plan(int64_t n, int64_t rows) {
-  int key_bits = 1;
-  while (key_bits < 32 && (rows >> key_bits) != 0) ++key_bits;  // rows itself is a key
-  SortPlan p;
-  p.passes = (key_bits + kDigitBits - 1) / kDigitBits;
-  p.bits = (key_bits + p.passes - 1) / p.passes;
-  p.blocks = (n + kSortTile - 1) / kSortTile;
-  auto up = [](size_t b) { return (b + 255) / 256 * 256; };
-  p.pair_bytes = p.passes > 1 ? up(size_t(n) * sizeof(uint2)) : 0;
-  p.count_bytes = up((size_t(1) << p.bits) * p.blocks * sizeof(uint32_t));
-  p.total_bytes = up((size_t(1) << p.bits) * sizeof(uint32_t));
-  return p;
-}
-
-// The pair at i: from the caller's indices in the first pass, else from the
-// pass before.
-__device__ __forceinline__ uint2 pair_at(const Index& index, const uint2* from, int64_t i) {
-  return from ? from[i] : make_uint2(row_of(index, i), uint32_t(i));
-}
-
-static __global__ void __launch_bounds__(kSortThreads)
-    count_kernel(int64_t n, Index index, const uint2* __restrict__ from, int shift, int bits,
-                 uint32_t* __restrict__ counts) {
-  __shared__ uint32_t bins[1 << kDigitBits];
-  const uint32_t mask = (1u << bits) - 1;
-  for (uint32_t d = threadIdx.x; d <= mask; d += kSortThreads) bins[d] = 0;
-  __syncthreads();
-  const int64_t base = int64_t(blockIdx.x) * kSortTile;
-  for (int j = 0; j < kSortItems; ++j) {
-    const int64_t i = base + j * kSortThreads + threadIdx.x;
-    if (i < n) {
-      const uint32_t key = from ? from[i].x : row_of(index, i);
-      atomicAdd(&bins[(key >> shift) & mask], 1u);
-    }
-  }
-  __syncthreads();
-  for (uint32_t d = threadIdx.x; d <= mask; d += kSortThreads)
-    counts[int64_t(d) * gridDim.x + blockIdx.x] = bins[d];
-}
-
-// One warp per digit: counts[d][blocks] to exclusive sums, totals[d] their sum.
-static __global__ void __launch_bounds__(kSortThreads)
-    scan_counts_kernel(int digits, int64_t blocks, uint32_t* __restrict__ counts,
-                       uint32_t* __restrict__ totals) {
-  const int d = int(blockIdx.x) * kSortWarps + int(threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (d >= digits) return;
-  uint32_t* row = counts + int64_t(d) * blocks;
-  uint32_t sum = 0;
-  for (int64_t at = 0; at < blocks; at += 32) {
-    const uint32_t mine = at + lane < blocks ? row[at + lane] : 0;
-    uint32_t inclusive = mine;
+// The tokens at `at(j)`, j < I, where that is below n: from the caller's indices
+// in the first pass, else from the pass before.
+template <int I, class At>
+__device__ __forceinline__ void load_pairs(const Index& index, const uint2* from, int64_t n, At at,
+                                           uint2 (&pair)[I]) {
+  if (from) {
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t below = __shfl_up_sync(~0u, inclusive, o);
-      if (lane >= o) inclusive += below;
-    }
-    if (at + lane < blocks) row[at + lane] = sum + inclusive - mine;
-    sum += __shfl_sync(~0u, inclusive, 31);
+    for (int j = 0; j < I; ++j)
+      if (at(j) < n) pair[j] = from[at(j)];
+    return;
   }
-  if (lane == 0) totals[d] = sum;
+  int64_t raw[I];
+#pragma unroll
+  for (int j = 0; j < I; ++j) raw[j] = at(j) < n ? raw_index(index, at(j)) : 0;
+#pragma unroll
+  for (int j = 0; j < I; ++j)
+    if (at(j) < n) pair[j] = make_uint2(row_of(index, raw[j]), uint32_t(at(j)));
 }
 
-static __global__ void __launch_bounds__(kSortThreads)
-    scatter_kernel(int64_t n, Index index, const uint2* __restrict__ from, int shift, int bits,
-                   const uint32_t* __restrict__ counts, const uint32_t* __restrict__ totals,
-                   uint2* __restrict__ to) {
-  __shared__ uint32_t warp_bins[kSortWarps][1 << kDigitBits];
-  __shared__ uint32_t warp_sums[kSortWarps];
+// Ranks of a tile: thread t of warp w holds the tokens w * 32 * I + 32 * j + lane,
+// j < I, the first `count` of the tile being real. bins: [warps][digits], zero
+// on entry; afterwards the tokens of each warp and digit. rank: how many tokens
+// of the same warp and digit stand before.
+template <int I>
+__device__ __forceinline__ void rank_tile(const uint2 (&pair)[I], int count, int shift, int bits,
+                                          uint16_t* bins, uint32_t (&rank)[I]) {
   const int digits = 1 << bits;
-  const uint32_t mask = uint32_t(digits) - 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int d = threadIdx.x; d < digits * kSortWarps; d += kSortThreads)
-    warp_bins[d / digits][d % digits] = 0;
-  __syncthreads();
-  // Ranks within the warp's share of the tile, in token order.
-  const int64_t base = int64_t(blockIdx.x) * kSortTile + warp * 32 * kSortItems + lane;
-  uint2 pair[kSortItems];
-  uint32_t rank[kSortItems];
+  uint16_t* mine = bins + warp * digits;
+  const int base = warp * 32 * I + lane;
+  // Lanes with an equal digit, by one ballot a bit (a match instruction took
+  // four times as long: 54 us against 13 for 16384 tokens in two passes).
+  uint32_t same[I];
 #pragma unroll
-  for (int j = 0; j < kSortItems; ++j) {
-    const int64_t i = base + 32 * j;
-    const bool real = i < n;
-    pair[j] = real ? pair_at(index, from, i) : make_uint2(0, 0);
-    const uint32_t digit = real ? (pair[j].x >> shift) & mask : ~0u;
-    const uint32_t same = __match_any_sync(~0u, digit);
-    const int leader = __ffs(same) - 1;
-    uint32_t before = 0;
-    if (lane == leader && real) {
-      before = warp_bins[warp][digit];
-      warp_bins[warp][digit] = before + __popc(same);
+  for (int j = 0; j < I; ++j) same[j] = __ballot_sync(~0u, base + 32 * j < count);
+  for (int b = shift; b < shift + bits; ++b) {
+#pragma unroll
+    for (int j = 0; j < I; ++j) {
+      const bool set = b < 32 && (pair[j].x >> b & 1);
+      const uint32_t lanes = __ballot_sync(~0u, set);
+      same[j] &= set ? lanes : ~lanes;
     }
-    rank[j] = __shfl_sync(~0u, before, leader) + __popc(same & ((1u << lane) - 1));
+  }
+#pragma unroll
+  for (int j = 0; j < I; ++j) {
+    const uint32_t digit = (pair[j].x >> shift) & (digits - 1);
+    const uint32_t below = __popc(same[j] & ((1u << lane) - 1));
+    uint32_t before = 0;
+    if (base + 32 * j < count) {
+      before = mine[digit];
+      rank[j] = before + below;
+    }
+    __syncwarp();
+    if (base + 32 * j < count && below == 0) mine[digit] = uint16_t(before + __popc(same[j]));
     __syncwarp();
   }
-  __syncthreads();
-  // Where each warp's tokens of a digit begin: all smaller digits, then this
-  // digit's earlier blocks, then its earlier warps.
-  const int each = (digits + kSortThreads - 1) / kSortThreads;
-  uint32_t mine = 0;
-  for (int k = 0; k < each; ++k) {
-    const int d = threadIdx.x * each + k;
-    if (d < digits) mine += totals[d];
-  }
-  uint32_t inclusive = mine;
+}
+
+// Exclusive sum over the block's threads of one value each; sums: one a warp.
+__device__ __forceinline__ uint32_t exclusive_sum(uint32_t value, uint32_t* sums) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint32_t inclusive = value;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const uint32_t below = __shfl_up_sync(~0u, inclusive, o);
     if (lane >= o) inclusive += below;
   }
-  if (lane == 31) warp_sums[warp] = inclusive;
+  if (lane == 31) sums[warp] = inclusive;
   __syncthreads();
-  uint32_t start = inclusive - mine;
-  for (int w = 0; w < warp; ++w) start += warp_sums[w];
+  uint32_t before = 0;
+  for (int w = 0; w < warp; ++w) before += sums[w];
+  return before + inclusive - value;
+}
+
+inline int key_bits(int64_t rows) {  // of the keys 0 to rows
+  int bits = 1;
+  while (bits < 32 && (rows >> bits) != 0) ++bits;
+  return bits;
+}
+
+// ---- one block ----
+
+constexpr int kSmallThreads = 1024;
+constexpr int kSmallWarps = kSmallThreads / 32;
+constexpr int kSmallBits = 9;
+constexpr int kSmall = kSmallThreads * 16;
+
+template <int I>
+__global__ void __launch_bounds__(kSmallThreads)
+    small_sort_kernel(int n, Index index, int passes, int bits, uint2* __restrict__ order) {
+  extern __shared__ __align__(16) char shared[];
+  uint2* pairs = reinterpret_cast<uint2*>(shared);                 // [I * threads]
+  uint16_t* bins = reinterpret_cast<uint16_t*>(pairs + I * kSmallThreads);  // [warps][digits]
+  const int digits = 1 << bits;
+  uint32_t* starts = reinterpret_cast<uint32_t*>(bins + kSmallWarps * digits);  // [digits]
+  uint32_t* sums = starts + digits;                                             // [warps]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int base = warp * 32 * I + lane;
+  uint2 pair[I];
+  uint32_t rank[I];
+  load_pairs<I>(index, nullptr, n, [&](int j) { return int64_t(base + 32 * j); }, pair);
+  for (int pass = 0; pass < passes; ++pass) {
+    const int shift = pass * bits;
+    for (int d = threadIdx.x; d < kSmallWarps * digits / 2; d += kSmallThreads)
+      reinterpret_cast<uint32_t*>(bins)[d] = 0;
+    __syncthreads();
+    rank_tile<I>(pair, n, shift, bits, bins, rank);
+    __syncthreads();
+    // Each warp's tokens of a digit among the digit's, then the digits' starts.
+    uint32_t total = 0;
+    if (int(threadIdx.x) < digits) {
+#pragma unroll 8
+      for (int w = 0; w < kSmallWarps; ++w) {
+        const uint32_t c = bins[w * digits + threadIdx.x];
+        bins[w * digits + threadIdx.x] = uint16_t(total);
+        total += c;
+      }
+    }
+    const uint32_t start = exclusive_sum(total, sums);
+    if (int(threadIdx.x) < digits) starts[threadIdx.x] = start;
+    __syncthreads();
+    const bool last = pass + 1 == passes;
+#pragma unroll
+    for (int j = 0; j < I; ++j)
+      if (base + 32 * j < n) {
+        const uint32_t digit = (pair[j].x >> shift) & (digits - 1);
+        const uint32_t at = starts[digit] + bins[warp * digits + digit] + rank[j];
+        (last ? order : pairs)[at] = pair[j];
+      }
+    if (last) break;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < I; ++j)
+      if (base + 32 * j < n) pair[j] = pairs[base + 32 * j];
+  }
+}
+
+template <int I>
+cudaError_t small_sort(int64_t n, const Index& index, uint2* order, cudaStream_t stream) {
+  const int all = key_bits(index.rows);
+  const int passes = (all + kSmallBits - 1) / kSmallBits, bits = (all + passes - 1) / passes;
+  const size_t shared = size_t(I) * kSmallThreads * sizeof(uint2) +
+                        (size_t(1) << bits) * (kSmallWarps * sizeof(uint16_t) + sizeof(uint32_t)) +
+                        kSmallWarps * sizeof(uint32_t);
+  const cudaError_t e = cudaFuncSetAttribute(
+      small_sort_kernel<I>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared));
+  if (e != cudaSuccess) return e;
+  small_sort_kernel<I><<<1, kSmallThreads, shared, stream>>>(int(n), index, passes, bits, order);
+  return cudaGetLastError();
+}
+
+// ---- many blocks ----
+
+constexpr int kSortThreads = 512;
+constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kSortBits = 11;
+constexpr int kSortBlocks = 148;
+
+struct SortPlan {
+  int items;         // tokens of a thread in a tile
+  int passes, bits;  // digit width of every pass
+  int blocks, tiles;  // blocks, and tiles of each
+  size_t pair_bytes, count_bytes;  // workspace parts
+
+  size_t bytes() const { return pair_bytes + count_bytes; }
+};
+
+inline SortPlan sort_plan(int64_t n, int64_t rows) {
+  SortPlan p{};
+  if (n <= kSmall) return p;
+  const int all = key_bits(rows);
+  p.passes = (all + kSortBits - 1) / kSortBits;
+  p.bits = (all + p.passes - 1) / p.passes;
+  // Small tiles while they leave no block more than one.
+  p.items = n <= int64_t(kSortBlocks) * kSortThreads * 4 ? 4 : 16;
+  const int64_t tiles = (n + kSortThreads * p.items - 1) / (kSortThreads * p.items);
+  p.tiles = int((tiles + kSortBlocks - 1) / kSortBlocks);
+  p.blocks = int((tiles + p.tiles - 1) / p.tiles);
+  auto up = [](size_t b) { return (b + 255) / 256 * 256; };
+  p.pair_bytes = p.passes > 1 ? up(size_t(n) * sizeof(uint2)) : 0;
+  p.count_bytes = up((size_t(1) << p.bits) * p.blocks * sizeof(uint32_t));
+  return p;
+}
+
+// counts[block][digit]
+template <int I>
+__global__ void __launch_bounds__(kSortThreads)
+    count_kernel(int64_t n, Index index, const uint2* __restrict__ from, int tiles, int shift,
+                 int bits, uint32_t* __restrict__ counts) {
+  __shared__ uint32_t bins[1 << kSortBits];
+  const int digits = 1 << bits;
+  for (int d = threadIdx.x; d < digits; d += kSortThreads) bins[d] = 0;
+  __syncthreads();
+  for (int t = 0; t < tiles; ++t) {
+    const int64_t base = (int64_t(blockIdx.x) * tiles + t) * (kSortThreads * I) + threadIdx.x;
+    uint2 pair[I];
+    load_pairs<I>(index, from, n, [&](int j) { return base + j * kSortThreads; }, pair);
+#pragma unroll
+    for (int j = 0; j < I; ++j)
+      if (base + j * kSortThreads < n) atomicAdd(&bins[(pair[j].x >> shift) & (digits - 1)], 1u);
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < digits; d += kSortThreads)
+    counts[int64_t(blockIdx.x) * digits + d] = bins[d];
+}
+
+template <int I>
+__global__ void __launch_bounds__(kSortThreads)
+    scatter_kernel(int64_t n, Index index, const uint2* __restrict__ from, int tiles, int shift,
+                   int bits, const uint32_t* __restrict__ counts, uint2* __restrict__ to) {
+  extern __shared__ __align__(16) char shared[];
+  const int digits = 1 << bits;
+  uint32_t* starts = reinterpret_cast<uint32_t*>(shared);               // [digits]
+  uint32_t* earlier = starts + digits;                                  // [digits]
+  uint16_t* bins = reinterpret_cast<uint16_t*>(earlier + digits);       // [warps][digits]
+  __shared__ uint32_t sums[kSortWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // Where this block's tokens of each digit begin: all smaller digits, then
+  // this digit's tokens of the blocks in front.
+  for (int d = threadIdx.x; d < 2 * digits; d += kSortThreads) starts[d] = 0;
+  __syncthreads();
+  const int parts = digits < kSortThreads ? kSortThreads / digits : 1;
+  for (int d = threadIdx.x % digits; d < digits; d += kSortThreads) {
+    uint32_t all = 0, front = 0;
+#pragma unroll 8
+    for (int b = threadIdx.x / digits % parts; b < int(gridDim.x); b += parts) {
+      const uint32_t c = counts[int64_t(b) * digits + d];
+      all += c;
+      if (b < int(blockIdx.x)) front += c;
+    }
+    atomicAdd(&starts[d], all);
+    atomicAdd(&earlier[d], front);
+  }
+  __syncthreads();
+  const int each = (digits + kSortThreads - 1) / kSortThreads;
+  uint32_t mine = 0;
+  for (int k = 0; k < each; ++k) {
+    const int d = threadIdx.x * each + k;
+    if (d < digits) mine += starts[d];
+  }
+  uint32_t start = exclusive_sum(mine, sums);
   for (int k = 0; k < each; ++k) {
     const int d = threadIdx.x * each + k;
     if (d >= digits) break;
-    uint32_t at = start + counts[int64_t(d) * gridDim.x + blockIdx.x];
-    for (int w = 0; w < kSortWarps; ++w) {
-      const uint32_t c = warp_bins[w][d];
-      warp_bins[w][d] = at;
-      at += c;
-    }
-    start += totals[d];
+    const uint32_t c = starts[d];
+    starts[d] = start + earlier[d];
+    start += c;
   }
-  __syncthreads();
+  for (int t = 0; t < tiles; ++t) {
+    const int64_t first = (int64_t(blockIdx.x) * tiles + t) * (kSortThreads * I);
+    if (first >= n) break;
+    const int count = int(n - first < kSortThreads * I ? n - first : kSortThreads * I);
+    const int base = warp * 32 * I + lane;
+    uint2 pair[I];
+    uint32_t rank[I];
+    load_pairs<I>(index, from, n, [&](int j) { return first + base + 32 * j; }, pair);
+    for (int d = threadIdx.x; d < kSortWarps * digits / 2; d += kSortThreads)
+      reinterpret_cast<uint32_t*>(bins)[d] = 0;
+    __syncthreads();
+    rank_tile<I>(pair, count, shift, bits, bins, rank);
+    __syncthreads();
+    for (int d = threadIdx.x; d < digits; d += kSortThreads) {
+      uint32_t total = 0;
 #pragma unroll
-  for (int j = 0; j < kSortItems; ++j)
-    if (base + 32 * j < n)
-      to[warp_bins[warp][(pair[j].x >> shift) & mask] + rank[j]] = pair[j];
+      for (int w = 0; w < kSortWarps; ++w) {
+        const uint32_t c = bins[w * digits + d];
+        bins[w * digits + d] = uint16_t(total);
+        total += c;
+      }
+      earlier[d] = total;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < I; ++j)
+      if (base + 32 * j < count) {
+        const uint32_t digit = (pair[j].x >> shift) & (digits - 1);
+        to[starts[digit] + bins[warp * digits + digit] + rank[j]] = pair[j];
+      }
+    __syncthreads();
+    for (int d = threadIdx.x; d < digits; d += kSortThreads) starts[d] += earlier[d];
+    // (the next tile's first barrier orders these sums before their use)
+  }
 }
 
-// Sorts into order[n]; workspace of sort_plan(n, rows).bytes().
-inline cudaError_t sort_tokens(int64_t n, const Index& index, uint2* order, void* workspace,
-                               cudaStream_t stream) {
-  const SortPlan p = sort_plan(n, index.rows);
-  char* at = static_cast<char*>(workspace);
-  uint2* spare = reinterpret_cast<uint2*>(at);
-  uint32_t* counts = reinterpret_cast<uint32_t*>(at + p.pair_bytes);
-  uint32_t* totals = reinterpret_cast<uint32_t*>(at + p.pair_bytes + p.count_bytes);
-  const unsigned blocks = unsigned(p.blocks);
+template <int I>
+cudaError_t large_sort(int64_t n, const Index& index, const SortPlan& p, uint2* order,
+                       void* workspace, cudaStream_t stream) {
+  uint2* spare = static_cast<uint2*>(workspace);
+  uint32_t* counts =
+      reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + p.pair_bytes);
+  const size_t shared =
+      (size_t(1) << p.bits) * (2 * sizeof(uint32_t) + kSortWarps * sizeof(uint16_t));
+  const cudaError_t e = cudaFuncSetAttribute(
+      scatter_kernel<I>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared));
+  if (e != cudaSuccess) return e;
   const uint2* from = nullptr;
   for (int pass = 0; pass < p.passes; ++pass) {
     // Alternating so that the last pass ends in `order`.
     uint2* to = (p.passes - 1 - pass) % 2 == 0 ? order : spare;
     const int shift = pass * p.bits;
-    count_kernel<<<blocks, kSortThreads, 0, stream>>>(n, index, from, shift, p.bits, counts);
-    scan_counts_kernel<<<((1 << p.bits) + kSortWarps - 1) / kSortWarps, kSortThreads, 0, stream>>>(
-        1 << p.bits, p.blocks, counts, totals);
-    scatter_kernel<<<blocks, kSortThreads, 0, stream>>>(n, index, from, shift, p.bits, counts,
-                                                        totals, to);
+    count_kernel<I><<<p.blocks, kSortThreads, 0, stream>>>(n, index, from, p.tiles, shift, p.bits,
+                                                           counts);
+    scatter_kernel<I><<<p.blocks, kSortThreads, shared, stream>>>(n, index, from, p.tiles, shift,
+                                                                  p.bits, counts, to);
     from = to;
   }
   return cudaGetLastError();
+}
+
+// Sorts into order[n]; workspace of sort_plan(n, rows).bytes() (none for few
+// tokens).
+inline cudaError_t sort_tokens(int64_t n, const Index& index, uint2* order, void* workspace,
+                               cudaStream_t stream) {
+  if (n <= kSmallThreads) return small_sort<1>(n, index, order, stream);
+  if (n <= kSmallThreads * 4) return small_sort<4>(n, index, order, stream);
+  if (n <= kSmall) return small_sort<16>(n, index, order, stream);
+  const SortPlan p = sort_plan(n, index.rows);
+  return p.items == 4 ? large_sort<4>(n, index, p, order, workspace, stream)
+                      : large_sort<16>(n, index, p, order, workspace, stream);
 }
 
 }  // namespace tokens

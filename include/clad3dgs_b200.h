@@ -508,8 +508,8 @@ int clad3dgs_dropout(int type, int64_t rows, int64_t width, const void* x, int64
  * int32 or int64 (index_bits); an index equal to `padding` (has_padding != 0)
  * names no row, nor does one outside [0, rows), which also sets a bit of the
  * fault word (clad3dgs_fault_status). n and rows below 2^31. workspace:
- * clad3dgs_token_order_workspace bytes, 256-byte aligned, free again when the
- * call's work on the stream is done. */
+ * clad3dgs_token_order_workspace bytes (0 for few tokens: then it may be null),
+ * 256-byte aligned, free again when the call's work on the stream is done. */
 size_t clad3dgs_token_order_workspace(int64_t n, int64_t rows);
 int clad3dgs_token_order(int64_t n, int64_t rows, const void* index, int index_bits,
                          int has_padding, int64_t padding, uint32_t* order, void* workspace,
