@@ -8,7 +8,6 @@
 // one rounding to the element type.
 #include <cuda_runtime.h>
 
-#include <algorithm>
 #include <cstdint>
 #include <string>
 
@@ -23,42 +22,188 @@ namespace {
 
 constexpr int kThreads = 256;
 
-template <class T, bool kRows>
+// Bound by moving the elements once each way; the generator's ten rounds serve
+// four elements and hide behind that while every access is 16 bytes. Vectors
+// of V elements, U of them a thread, all loaded before the first is drawn for.
+
+// Packed rows: element numbers are addresses.
+template <class T, int V, int U>
 __global__ void __launch_bounds__(kThreads)
-    dropout_kernel(int64_t n, int64_t width, const T* x, int64_t x_stride, T* y,
-                   int64_t y_stride, float factor, CounterMask mask) {
+    packed_kernel(int64_t n, const T* x, T* y, float factor, CounterMask mask) {
   const unsigned long long offset = mask_offset(mask);
-  const int64_t blocks = (n + 3) / 4;
-  for (int64_t b = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; b < blocks;
-       b += (int64_t)gridDim.x * blockDim.x) {
-    uint4 words = make_uint4(0, 0, 0, 0);
-    if (!kRows) words = mask_words(mask, offset, b);
-    int64_t row = 4 * b / width, column = 4 * b - row * width;
-    const int count = int(n - 4 * b < 4 ? n - 4 * b : 4);
-    for (int j = 0; j < count; ++j) {
-      const uint32_t word =
-          kRows ? word_of(mask_words(mask, offset, row / 4), row % 4) : word_of(words, j);
-      const float v = to_float(x[row * x_stride + column]) * factor;
-      y[row * y_stride + column] = from_float<T>(mask.keeps(word) ? v : 0.f);
-      if (++column == width) column = 0, ++row;
-    }
+  const int64_t first = (int64_t(blockIdx.x) * (U * kThreads) + threadIdx.x) * V;
+  constexpr int64_t kApart = int64_t(kThreads) * V;
+  Vec<T, V> v[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t at = first + u * kApart;
+    if (at + V <= n) v[u] = *reinterpret_cast<const Vec<T, V>*>(x + at);
+    else
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (at + j < n) v[u].v[j] = x[at + j];
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t at = first + u * kApart;
+    if (at >= n) return;
+    bool keep[V];
+    mask_vector<V>(mask, offset, at, keep);
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      v[u].v[j] = from_float<T>(keep[j] ? to_float(v[u].v[j]) * factor : 0.f);
+    if (at + V <= n) *reinterpret_cast<Vec<T, V>*>(y + at) = v[u];
+    else
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (at + j < n) y[at + j] = v[u].v[j];
   }
 }
 
-template <class T>
-cudaError_t launch(int64_t rows, int64_t width, const void* x, int64_t x_stride, void* y,
-                   int64_t y_stride, double p, uint64_t seed, uint64_t offset,
-                   const int64_t* offset_device, bool by_row, cudaStream_t stream) {
-  const int64_t n = rows * width;
-  const CounterMask mask =
-      counter_mask(p, seed, offset, reinterpret_cast<const long long*>(offset_device));
-  const float factor = float(1.0 / (1.0 - p));
-  const unsigned grid =
-      unsigned(std::min<int64_t>((n / 4 + kThreads) / kThreads, int64_t(1) << 20));
-  auto* kernel = by_row ? dropout_kernel<T, true> : dropout_kernel<T, false>;
-  kernel<<<grid, kThreads, 0, stream>>>(n, width, static_cast<const T*>(x), x_stride,
-                                        static_cast<T*>(y), y_stride, factor, mask);
+// Rows of whole vectors, with any stride that keeps them aligned; `vectors` a
+// row. kRows: one decision for each row.
+template <class T, class Number, int V, int U, bool kRows>
+__global__ void __launch_bounds__(kThreads)
+    aligned_rows_kernel(Number total, Number vectors, const T* x, int64_t x_stride, T* y,
+                        int64_t y_stride, float factor, CounterMask mask) {
+  const unsigned long long offset = mask_offset(mask);
+  const Number first = Number(blockIdx.x) * (U * kThreads) + threadIdx.x;
+  Vec<T, V> v[U];
+  Number row[U], column[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const Number at = first + u * kThreads;
+    row[u] = at / vectors;
+    column[u] = (at - row[u] * vectors) * V;
+    if (at < total) v[u] = *reinterpret_cast<const Vec<T, V>*>(x + row[u] * x_stride + column[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (first + u * kThreads >= total) return;
+    bool keep[V];
+    if constexpr (kRows) {
+      const bool kept =
+          mask.keeps(word_of(mask_words(mask, offset, row[u] / 4), unsigned(row[u] % 4)));
+#pragma unroll
+      for (int j = 0; j < V; ++j) keep[j] = kept;
+    } else {
+      mask_vector<V>(mask, offset, int64_t(first + u * kThreads) * V, keep);
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      v[u].v[j] = from_float<T>(keep[j] ? to_float(v[u].v[j]) * factor : 0.f);
+    *reinterpret_cast<Vec<T, V>*>(y + row[u] * y_stride + column[u]) = v[u];
+  }
+}
+
+// Any rows: V consecutive elements a thread, loaded one by one (neighbours hit
+// the same lines) and stored as a vector where the output is packed and
+// aligned (kPacked).
+template <class T, class Number, int V, bool kRows, bool kPacked>
+__global__ void __launch_bounds__(kThreads)
+    any_rows_kernel(Number total, Number width, const T* x, int64_t x_stride, T* y,
+                    int64_t y_stride, float factor, CounterMask mask) {
+  const unsigned long long offset = mask_offset(mask);
+  const Number at = (Number(blockIdx.x) * kThreads + threadIdx.x) * V;
+  if (at >= total) return;
+  const Number row = at / width, column = at - row * width;
+  Vec<T, V> v;
+  {
+    Number r = row, c = column;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (c == width) c = 0, ++r;
+      if (at + j < total) v.v[j] = x[r * x_stride + c];
+      ++c;
+    }
+  }
+  bool keep[V];
+  if constexpr (kRows) {
+    Number r = row, c = column;
+    uint4 words = mask_words(mask, offset, r / 4);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (c == width) {
+        c = 0;
+        if (++r % 4 == 0) words = mask_words(mask, offset, r / 4);
+      }
+      keep[j] = mask.keeps(word_of(words, unsigned(r % 4)));
+      ++c;
+    }
+  } else {
+    mask_vector<V>(mask, offset, at, keep);
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+    v.v[j] = from_float<T>(keep[j] ? to_float(v.v[j]) * factor : 0.f);
+  if (kPacked && at + V <= total) {
+    *reinterpret_cast<Vec<T, V>*>(y + at) = v;
+    return;
+  }
+  Number r = row, c = column;
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    if (c == width) c = 0, ++r;
+    if (at + j < total) y[r * y_stride + c] = v.v[j];
+    ++c;
+  }
+}
+
+struct Call {
+  int64_t rows, width;
+  const void* x;
+  int64_t x_stride;
+  void* y;
+  int64_t y_stride;
+  float factor;
+  CounterMask mask;
+  bool by_row;
+  cudaStream_t stream;
+};
+
+unsigned grid_of(int64_t work, int64_t each) { return unsigned((work + each - 1) / each); }
+
+template <class T, class Number>
+cudaError_t launch_rows(const Call& a, bool aligned) {
+  constexpr int V = 16 / sizeof(T), U = 2;
+  const T* x = static_cast<const T*>(a.x);
+  T* y = static_cast<T*>(a.y);
+  if (aligned) {
+    const int64_t vectors = a.width / V, total = a.rows * vectors;
+    auto* kernel = a.by_row ? aligned_rows_kernel<T, Number, V, U, true>
+                            : aligned_rows_kernel<T, Number, V, U, false>;
+    kernel<<<grid_of(total, U * kThreads), kThreads, 0, a.stream>>>(
+        Number(total), Number(vectors), x, a.x_stride, y, a.y_stride, a.factor, a.mask);
+    return cudaGetLastError();
+  }
+  const int64_t total = a.rows * a.width;
+  const bool packed = (a.y_stride == a.width || a.rows == 1) && uint64_t(y) % 16 == 0;
+  auto* kernel = packed ? (a.by_row ? any_rows_kernel<T, Number, V, true, true>
+                                    : any_rows_kernel<T, Number, V, false, true>)
+                        : (a.by_row ? any_rows_kernel<T, Number, V, true, false>
+                                    : any_rows_kernel<T, Number, V, false, false>);
+  kernel<<<grid_of(total, V * kThreads), kThreads, 0, a.stream>>>(
+      Number(total), Number(a.width), x, a.x_stride, y, a.y_stride, a.factor, a.mask);
   return cudaGetLastError();
+}
+
+template <class T>
+cudaError_t launch(const Call& a) {
+  constexpr int V = 16 / sizeof(T), U = 2;
+  const int64_t n = a.rows * a.width;
+  const bool packed = a.rows == 1 || (a.x_stride == a.width && a.y_stride == a.width);
+  const bool based = (uint64_t(a.x) | uint64_t(a.y)) % 16 == 0;
+  // Rows of one element are decided one by one either way.
+  if (packed && based && (!a.by_row || a.width == 1)) {
+    packed_kernel<T, V, U><<<grid_of(n, int64_t(U) * V * kThreads), kThreads, 0, a.stream>>>(
+        n, static_cast<const T*>(a.x), static_cast<T*>(a.y), a.factor, a.mask);
+    return cudaGetLastError();
+  }
+  const bool aligned =
+      based && a.width % V == 0 && (a.rows == 1 || (a.x_stride % V == 0 && a.y_stride % V == 0));
+  // Divisions of 32-bit numbers while every element number fits one.
+  return n < (int64_t(1) << 32) - 2 * V * kThreads ? launch_rows<T, uint32_t>(a, aligned)
+                                                   : launch_rows<T, int64_t>(a, aligned);
 }
 
 }  // namespace
@@ -81,20 +226,13 @@ extern "C" int clad3dgs_dropout(int type, int64_t rows, int64_t width, const voi
   if (!x || !y) return fail(CLAD3DGS_INVALID_ARGUMENT, "dropout: null array");
   if (x_stride < 0 || (rows > 1 && y_stride < width))
     return fail(CLAD3DGS_INVALID_ARGUMENT, "dropout: bad row stride");
-  cudaError_t e;
-  switch (type) {
-    case CLAD3DGS_F32:
-      e = launch<float>(rows, width, x, x_stride, y, y_stride, p, seed, offset, offset_device,
-                        by_row != 0, stream);
-      break;
-    case CLAD3DGS_F16:
-      e = launch<__half>(rows, width, x, x_stride, y, y_stride, p, seed, offset, offset_device,
-                         by_row != 0, stream);
-      break;
-    default:
-      e = launch<__nv_bfloat16>(rows, width, x, x_stride, y, y_stride, p, seed, offset,
-                                offset_device, by_row != 0, stream);
-  }
+  const Call a{rows, width, x, x_stride, y, y_stride,
+               p < 1.0 ? float(1.0 / (1.0 - p)) : 0.f,
+               counter_mask(p, seed, offset, reinterpret_cast<const long long*>(offset_device)),
+               by_row != 0, stream};
+  const cudaError_t e = type == CLAD3DGS_F32   ? launch<float>(a)
+                        : type == CLAD3DGS_F16 ? launch<__half>(a)
+                                               : launch<__nv_bfloat16>(a);
   return e == cudaSuccess
              ? CLAD3DGS_OK
              : fail(CLAD3DGS_CUDA_ERROR, std::string("dropout: ") + cudaGetErrorString(e));

@@ -7,13 +7,15 @@
 // hold equal digits, in token order, so the sort is stable and the order the
 // same on every run.
 //
-// Up to kSmall tokens: one block sorts in shared memory, all passes in one
-// launch. More: two kernels a pass; every block (one an SM at most) counts the
-// digits of a contiguous share of the tokens, then adds up the other blocks'
-// counts itself (they lie in L2) and scatters its share tile by tile. Bound by
-// latency at these sizes: everything a thread reads of a tile is asked for
-// before any of it is used.
+// Up to kSmall tokens: one cluster of up to eight blocks sorts in shared memory,
+// all passes in one launch; blocks read each other's digit counts and scatter
+// into each other's tiles. More: two kernels a pass; every block (one an SM at
+// most) counts the digits of a contiguous share of the tokens, then adds up
+// the other blocks' counts itself (they lie in L2) and scatters its share tile
+// by tile. Bound by latency at these sizes: everything a thread reads of a tile
+// is asked for before any of it is used.
 #pragma once
+#include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -79,7 +81,7 @@ __device__ __forceinline__ void rank_tile(const uint2 (&pair)[I], int count, int
   uint16_t* mine = bins + warp * digits;
   const int base = warp * 32 * I + lane;
   // Lanes with an equal digit, by one ballot a bit (a match instruction took
-  // four times as long: 54 us against 13 for 16384 tokens in two passes).
+  // half as long again: 53 us against 37 for 16384 tokens in one block).
   uint32_t same[I];
 #pragma unroll
   for (int j = 0; j < I; ++j) same[j] = __ballot_sync(~0u, base + 32 * j < count);
@@ -128,81 +130,113 @@ inline int key_bits(int64_t rows) {  // of the keys 0 to rows
   return bits;
 }
 
-// ---- one block ----
+constexpr int kSortThreads = 1024;
+constexpr int kSortWarps = kSortThreads / 32;
 
-constexpr int kSmallThreads = 1024;
-constexpr int kSmallWarps = kSmallThreads / 32;
-constexpr int kSmallBits = 9;
-constexpr int kSmall = kSmallThreads * 16;
+// ---- one cluster ----
 
+constexpr int kClusterBits = 9;
+constexpr int kMostBlocks = 8;  // of a cluster
+constexpr int kSmall = kMostBlocks * kSortThreads * 8;
+
+// Block r of the cluster holds the tokens [r * tile, (r + 1) * tile) of the list
+// as sorted so far, tile = I * kSortThreads.
 template <int I>
-__global__ void __launch_bounds__(kSmallThreads)
-    small_sort_kernel(int n, Index index, int passes, int bits, uint2* __restrict__ order) {
+__global__ void __launch_bounds__(kSortThreads)
+    cluster_sort_kernel(int n, Index index, int passes, int bits, uint2* __restrict__ order) {
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int blocks = int(cluster.num_blocks()), me = int(cluster.block_rank());
+  constexpr int kTile = I * kSortThreads;
   extern __shared__ __align__(16) char shared[];
-  uint2* pairs = reinterpret_cast<uint2*>(shared);                 // [I * threads]
-  uint16_t* bins = reinterpret_cast<uint16_t*>(pairs + I * kSmallThreads);  // [warps][digits]
   const int digits = 1 << bits;
-  uint32_t* starts = reinterpret_cast<uint32_t*>(bins + kSmallWarps * digits);  // [digits]
-  uint32_t* sums = starts + digits;                                             // [warps]
+  uint2* pairs = reinterpret_cast<uint2*>(shared);                    // [tile]
+  uint32_t* counts = reinterpret_cast<uint32_t*>(pairs + kTile);      // [digits]
+  uint32_t* starts = counts + digits;                                 // [digits]
+  uint16_t* bins = reinterpret_cast<uint16_t*>(starts + digits);      // [warps][digits]
+  __shared__ uint32_t sums[kSortWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int base = warp * 32 * I + lane;
+  const int first = me * kTile;
+  const int count = n - first < kTile ? n - first : kTile;
   uint2 pair[I];
   uint32_t rank[I];
-  load_pairs<I>(index, nullptr, n, [&](int j) { return int64_t(base + 32 * j); }, pair);
+  load_pairs<I>(index, nullptr, n, [&](int j) { return int64_t(first + base + 32 * j); }, pair);
   for (int pass = 0; pass < passes; ++pass) {
     const int shift = pass * bits;
-    for (int d = threadIdx.x; d < kSmallWarps * digits / 2; d += kSmallThreads)
+    for (int d = threadIdx.x; d < kSortWarps * digits / 2; d += kSortThreads)
       reinterpret_cast<uint32_t*>(bins)[d] = 0;
     __syncthreads();
-    rank_tile<I>(pair, n, shift, bits, bins, rank);
+    rank_tile<I>(pair, count, shift, bits, bins, rank);
     __syncthreads();
-    // Each warp's tokens of a digit among the digit's, then the digits' starts.
-    uint32_t total = 0;
-    if (int(threadIdx.x) < digits) {
+    // Each warp's tokens of a digit among the block's.
+    const int d = threadIdx.x;
+    if (d < digits) {
+      uint32_t total = 0;
 #pragma unroll 8
-      for (int w = 0; w < kSmallWarps; ++w) {
-        const uint32_t c = bins[w * digits + threadIdx.x];
-        bins[w * digits + threadIdx.x] = uint16_t(total);
+      for (int w = 0; w < kSortWarps; ++w) {
+        const uint32_t c = bins[w * digits + d];
+        bins[w * digits + d] = uint16_t(total);
         total += c;
       }
+      counts[d] = total;
     }
-    const uint32_t start = exclusive_sum(total, sums);
-    if (int(threadIdx.x) < digits) starts[threadIdx.x] = start;
+    cluster.sync();  // all counts are there, and all tiles are in registers
+    uint32_t all = 0, front = 0;
+    if (d < digits) {
+      for (int r = 0; r < blocks; ++r) {
+        const uint32_t c = cluster.map_shared_rank(counts, r)[d];
+        all += c;
+        if (r < me) front += c;
+      }
+    }
+    const uint32_t start = exclusive_sum(all, sums);
+    if (d < digits) starts[d] = start + front;
     __syncthreads();
     const bool last = pass + 1 == passes;
 #pragma unroll
     for (int j = 0; j < I; ++j)
-      if (base + 32 * j < n) {
+      if (base + 32 * j < count) {
         const uint32_t digit = (pair[j].x >> shift) & (digits - 1);
         const uint32_t at = starts[digit] + bins[warp * digits + digit] + rank[j];
-        (last ? order : pairs)[at] = pair[j];
+        if (last) order[at] = pair[j];
+        else cluster.map_shared_rank(pairs, at / kTile)[at % kTile] = pair[j];
       }
+    cluster.sync();  // the tiles are complete, and nobody reads a block that is gone
     if (last) break;
-    __syncthreads();
 #pragma unroll
     for (int j = 0; j < I; ++j)
-      if (base + 32 * j < n) pair[j] = pairs[base + 32 * j];
+      if (base + 32 * j < count) pair[j] = pairs[base + 32 * j];
   }
 }
 
 template <int I>
-cudaError_t small_sort(int64_t n, const Index& index, uint2* order, cudaStream_t stream) {
+cudaError_t cluster_sort(int64_t n, const Index& index, uint2* order, cudaStream_t stream) {
   const int all = key_bits(index.rows);
-  const int passes = (all + kSmallBits - 1) / kSmallBits, bits = (all + passes - 1) / passes;
-  const size_t shared = size_t(I) * kSmallThreads * sizeof(uint2) +
-                        (size_t(1) << bits) * (kSmallWarps * sizeof(uint16_t) + sizeof(uint32_t)) +
-                        kSmallWarps * sizeof(uint32_t);
-  const cudaError_t e = cudaFuncSetAttribute(
-      small_sort_kernel<I>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared));
+  const int passes = (all + kClusterBits - 1) / kClusterBits, bits = (all + passes - 1) / passes;
+  unsigned blocks = 1;
+  while (int64_t(blocks) * I * kSortThreads < n) blocks *= 2;
+  const size_t shared = size_t(I) * kSortThreads * sizeof(uint2) +
+                        (size_t(1) << bits) * (kSortWarps * sizeof(uint16_t) + 2 * sizeof(uint32_t));
+  cudaError_t e = cudaFuncSetAttribute(cluster_sort_kernel<I>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared));
   if (e != cudaSuccess) return e;
-  small_sort_kernel<I><<<1, kSmallThreads, shared, stream>>>(int(n), index, passes, bits, order);
-  return cudaGetLastError();
+  cudaLaunchAttribute attribute{};
+  attribute.id = cudaLaunchAttributeClusterDimension;
+  attribute.val.clusterDim.x = blocks;
+  attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(blocks);
+  config.blockDim = dim3(kSortThreads);
+  config.dynamicSmemBytes = shared;
+  config.stream = stream;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, cluster_sort_kernel<I>, int(n), index, passes, bits, order);
 }
 
 // ---- many blocks ----
 
-constexpr int kSortThreads = 512;
-constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kSortBits = 11;
 constexpr int kSortBlocks = 148;
 
@@ -222,7 +256,7 @@ inline SortPlan sort_plan(int64_t n, int64_t rows) {
   p.passes = (all + kSortBits - 1) / kSortBits;
   p.bits = (all + p.passes - 1) / p.passes;
   // Small tiles while they leave no block more than one.
-  p.items = n <= int64_t(kSortBlocks) * kSortThreads * 4 ? 4 : 16;
+  p.items = n <= int64_t(kSortBlocks) * kSortThreads * 2 ? 2 : 8;
   const int64_t tiles = (n + kSortThreads * p.items - 1) / (kSortThreads * p.items);
   p.tiles = int((tiles + kSortBlocks - 1) / kSortBlocks);
   p.blocks = int((tiles + p.tiles - 1) / p.tiles);
@@ -361,12 +395,14 @@ cudaError_t large_sort(int64_t n, const Index& index, const SortPlan& p, uint2* 
 // tokens).
 inline cudaError_t sort_tokens(int64_t n, const Index& index, uint2* order, void* workspace,
                                cudaStream_t stream) {
-  if (n <= kSmallThreads) return small_sort<1>(n, index, order, stream);
-  if (n <= kSmallThreads * 4) return small_sort<4>(n, index, order, stream);
-  if (n <= kSmall) return small_sort<16>(n, index, order, stream);
+  // As many blocks as give each thread one token, then more tokens a thread.
+  if (n <= kSmall / 8) return cluster_sort<1>(n, index, order, stream);
+  if (n <= kSmall / 4) return cluster_sort<2>(n, index, order, stream);
+  if (n <= kSmall / 2) return cluster_sort<4>(n, index, order, stream);
+  if (n <= kSmall) return cluster_sort<8>(n, index, order, stream);
   const SortPlan p = sort_plan(n, index.rows);
-  return p.items == 4 ? large_sort<4>(n, index, p, order, workspace, stream)
-                      : large_sort<16>(n, index, p, order, workspace, stream);
+  return p.items == 2 ? large_sort<2>(n, index, p, order, workspace, stream)
+                      : large_sort<8>(n, index, p, order, workspace, stream);
 }
 
 }  // namespace tokens
