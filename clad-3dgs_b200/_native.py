@@ -121,7 +121,7 @@ _SIGNATURES = {
     "clad3dgs_embedding_lookup": (c_int, [c_int, c_int64, c_int64, c_int64, _P, c_int64, _P,
                                           c_int, c_int, c_int64, c_double, c_double, c_uint64,
                                           c_uint64, _P, _P, _P]),
-    "clad3dgs_embedding_workspace": (c_size_t, [c_int64, c_int64]),
+    "clad3dgs_embedding_workspace": (c_size_t, [c_int64, c_int64, c_int64, c_int]),
     "clad3dgs_embedding_gradient": (c_int, [c_int, c_int64, c_int64, c_int64, _P, c_int64, _P,
                                             c_double, c_double, c_uint64, c_uint64, _P, _P, _P,
                                             c_size_t, _P]),

@@ -15,10 +15,14 @@
 
 namespace clad3dgs {
 
+constexpr int kMaskRounds = 10;
+
 // One dropout as a kernel argument: kept iff word >= limit, for p < 1; `none`
-// keeps nothing (p = 1, whose limit does not fit a word).
+// keeps nothing (p = 1, whose limit does not fit a word). The rounds' keys are
+// made on the host, so that a round is two products and two three-way
+// exclusive-ors with one operand from the argument.
 struct CounterMask {
-  uint32_t key0, key1;
+  uint32_t key0[kMaskRounds], key1[kMaskRounds];
   unsigned long long offset;
   const long long* offset_device;  // nullable: added to offset by the kernel
   uint32_t limit;
@@ -30,8 +34,10 @@ struct CounterMask {
 inline CounterMask counter_mask(double p, uint64_t seed, uint64_t offset,
                                 const long long* offset_device) {
   CounterMask m;
-  m.key0 = uint32_t(seed);
-  m.key1 = uint32_t(seed >> 32);
+  for (int r = 0; r < kMaskRounds; ++r) {
+    m.key0[r] = uint32_t(seed) + uint32_t(r) * 0x9E3779B9u;
+    m.key1[r] = uint32_t(seed >> 32) + uint32_t(r) * 0xBB67AE85u;
+  }
   m.offset = offset;
   m.offset_device = offset_device;
   m.none = p >= 1.0;
@@ -43,20 +49,21 @@ __device__ __forceinline__ unsigned long long mask_offset(const CounterMask& m) 
   return m.offset + (m.offset_device ? (unsigned long long)*m.offset_device : 0ull);
 }
 
+// The four words of a block of four elements. Number: uint32_t where every block
+// number fits one (its high half is then a constant zero).
+template <class Number>
 __device__ __forceinline__ uint4 mask_words(const CounterMask& m, unsigned long long offset,
-                                            unsigned long long block) {
-  uint32_t c0 = uint32_t(block), c1 = uint32_t(block >> 32), c2 = uint32_t(offset),
-           c3 = uint32_t(offset >> 32), k0 = m.key0, k1 = m.key1;
+                                            Number block) {
+  uint32_t c0 = uint32_t(block), c1 = sizeof(Number) > 4 ? uint32_t(uint64_t(block) >> 32) : 0u,
+           c2 = uint32_t(offset), c3 = uint32_t(offset >> 32);
 #pragma unroll
-  for (int r = 0; r < 10; ++r) {
+  for (int r = 0; r < kMaskRounds; ++r) {
     const unsigned long long a = (unsigned long long)0xD2511F53u * c0;
     const unsigned long long b = (unsigned long long)0xCD9E8D57u * c2;
-    c0 = uint32_t(b >> 32) ^ c1 ^ k0;
+    c0 = uint32_t(b >> 32) ^ c1 ^ m.key0[r];
     c1 = uint32_t(b);
-    c2 = uint32_t(a >> 32) ^ c3 ^ k1;
+    c2 = uint32_t(a >> 32) ^ c3 ^ m.key1[r];
     c3 = uint32_t(a);
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
   }
   return make_uint4(c0, c1, c2, c3);
 }
@@ -65,15 +72,23 @@ __device__ __forceinline__ uint32_t word_of(const uint4& w, unsigned j) {
   return j == 0 ? w.x : j == 1 ? w.y : j == 2 ? w.z : w.w;
 }
 
-// The decisions for V elements that begin at element e.
-template <int V>
+// The decisions for V elements that begin at element e, e a multiple of V (a
+// multiple of four, or V = 1). Number: uint32_t where every e / 4 fits one.
+template <int V, class Number = uint64_t>
 __device__ __forceinline__ void mask_vector(const CounterMask& m, unsigned long long offset,
-                                            int64_t e, bool (&keep)[V]) {
-  uint4 words = mask_words(m, offset, e / 4);
+                                            uint64_t e, bool (&keep)[V]) {
+  static_assert(V == 1 || V % 4 == 0, "whole blocks, or one element");
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    if (j > 0 && (e + j) % 4 == 0) words = mask_words(m, offset, (e + j) / 4);
-    keep[j] = m.keeps(word_of(words, unsigned(e + j) % 4));
+  for (int j = 0; j < V; j += 4) {
+    const uint4 words = mask_words(m, offset, Number((e + j) / 4));
+    if constexpr (V == 1) {
+      keep[0] = m.keeps(word_of(words, unsigned(e) % 4));
+    } else {
+      keep[j] = m.keeps(words.x);
+      keep[j + 1] = m.keeps(words.y);
+      keep[j + 2] = m.keeps(words.z);
+      keep[j + 3] = m.keeps(words.w);
+    }
   }
 }
 

@@ -27,9 +27,10 @@ constexpr int kThreads = 256;
 // of V elements, U of them a thread, all loaded before the first is drawn for.
 
 // Packed rows: element numbers are addresses.
-template <class T, int V, int U>
+template <class T, class Number, int V, int U>
 __global__ void __launch_bounds__(kThreads)
-    packed_kernel(int64_t n, const T* x, T* y, float factor, CounterMask mask) {
+    packed_kernel(int64_t n, const T* x, T* y, float factor,
+                  const __grid_constant__ CounterMask mask) {
   const unsigned long long offset = mask_offset(mask);
   const int64_t first = (int64_t(blockIdx.x) * (U * kThreads) + threadIdx.x) * V;
   constexpr int64_t kApart = int64_t(kThreads) * V;
@@ -48,7 +49,7 @@ __global__ void __launch_bounds__(kThreads)
     const int64_t at = first + u * kApart;
     if (at >= n) return;
     bool keep[V];
-    mask_vector<V>(mask, offset, at, keep);
+    mask_vector<V, Number>(mask, offset, at, keep);
 #pragma unroll
     for (int j = 0; j < V; ++j)
       v[u].v[j] = from_float<T>(keep[j] ? to_float(v[u].v[j]) * factor : 0.f);
@@ -62,10 +63,12 @@ __global__ void __launch_bounds__(kThreads)
 
 // Rows of whole vectors, with any stride that keeps them aligned; `vectors` a
 // row. kRows: one decision for each row.
-template <class T, class Number, int V, int U, bool kRows>
+template <class T, class Division, int V, int U, bool kRows>
 __global__ void __launch_bounds__(kThreads)
-    aligned_rows_kernel(Number total, Number vectors, const T* x, int64_t x_stride, T* y,
-                        int64_t y_stride, float factor, CounterMask mask) {
+    aligned_rows_kernel(typename Division::Number total, const Division vectors, const T* x,
+                        int64_t x_stride, T* y, int64_t y_stride, float factor,
+                        const __grid_constant__ CounterMask mask) {
+  using Number = typename Division::Number;
   const unsigned long long offset = mask_offset(mask);
   const Number first = Number(blockIdx.x) * (U * kThreads) + threadIdx.x;
   Vec<T, V> v[U];
@@ -73,8 +76,8 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const Number at = first + u * kThreads;
-    row[u] = at / vectors;
-    column[u] = (at - row[u] * vectors) * V;
+    row[u] = vectors.quotient(at);
+    column[u] = (at - row[u] * vectors.divisor) * V;
     if (at < total) v[u] = *reinterpret_cast<const Vec<T, V>*>(x + row[u] * x_stride + column[u]);
   }
 #pragma unroll
@@ -87,7 +90,7 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
       for (int j = 0; j < V; ++j) keep[j] = kept;
     } else {
-      mask_vector<V>(mask, offset, int64_t(first + u * kThreads) * V, keep);
+      mask_vector<V>(mask, offset, uint64_t(first + u * kThreads) * V, keep);
     }
 #pragma unroll
     for (int j = 0; j < V; ++j)
@@ -99,20 +102,22 @@ __global__ void __launch_bounds__(kThreads)
 // Any rows: V consecutive elements a thread, loaded one by one (neighbours hit
 // the same lines) and stored as a vector where the output is packed and
 // aligned (kPacked).
-template <class T, class Number, int V, bool kRows, bool kPacked>
+template <class T, class Division, int V, bool kRows, bool kPacked>
 __global__ void __launch_bounds__(kThreads)
-    any_rows_kernel(Number total, Number width, const T* x, int64_t x_stride, T* y,
-                    int64_t y_stride, float factor, CounterMask mask) {
+    any_rows_kernel(typename Division::Number total, const Division width, const T* x,
+                    int64_t x_stride, T* y, int64_t y_stride, float factor,
+                    const __grid_constant__ CounterMask mask) {
+  using Number = typename Division::Number;
   const unsigned long long offset = mask_offset(mask);
   const Number at = (Number(blockIdx.x) * kThreads + threadIdx.x) * V;
   if (at >= total) return;
-  const Number row = at / width, column = at - row * width;
+  const Number row = width.quotient(at), column = at - row * width.divisor;
   Vec<T, V> v;
   {
     Number r = row, c = column;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      if (c == width) c = 0, ++r;
+      if (c == width.divisor) c = 0, ++r;
       if (at + j < total) v.v[j] = x[r * x_stride + c];
       ++c;
     }
@@ -123,7 +128,7 @@ __global__ void __launch_bounds__(kThreads)
     uint4 words = mask_words(mask, offset, r / 4);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      if (c == width) {
+      if (c == width.divisor) {
         c = 0;
         if (++r % 4 == 0) words = mask_words(mask, offset, r / 4);
       }
@@ -131,7 +136,7 @@ __global__ void __launch_bounds__(kThreads)
       ++c;
     }
   } else {
-    mask_vector<V>(mask, offset, at, keep);
+    mask_vector<V, Number>(mask, offset, at, keep);
   }
 #pragma unroll
   for (int j = 0; j < V; ++j)
@@ -143,7 +148,7 @@ __global__ void __launch_bounds__(kThreads)
   Number r = row, c = column;
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    if (c == width) c = 0, ++r;
+    if (c == width.divisor) c = 0, ++r;
     if (at + j < total) y[r * y_stride + c] = v.v[j];
     ++c;
   }
@@ -163,27 +168,28 @@ struct Call {
 
 unsigned grid_of(int64_t work, int64_t each) { return unsigned((work + each - 1) / each); }
 
-template <class T, class Number>
+template <class T, class Division>
 cudaError_t launch_rows(const Call& a, bool aligned) {
+  using Number = typename Division::Number;
   constexpr int V = 16 / sizeof(T), U = 2;
   const T* x = static_cast<const T*>(a.x);
   T* y = static_cast<T*>(a.y);
   if (aligned) {
     const int64_t vectors = a.width / V, total = a.rows * vectors;
-    auto* kernel = a.by_row ? aligned_rows_kernel<T, Number, V, U, true>
-                            : aligned_rows_kernel<T, Number, V, U, false>;
+    auto* kernel = a.by_row ? aligned_rows_kernel<T, Division, V, U, true>
+                            : aligned_rows_kernel<T, Division, V, U, false>;
     kernel<<<grid_of(total, U * kThreads), kThreads, 0, a.stream>>>(
-        Number(total), Number(vectors), x, a.x_stride, y, a.y_stride, a.factor, a.mask);
+        Number(total), Division(vectors), x, a.x_stride, y, a.y_stride, a.factor, a.mask);
     return cudaGetLastError();
   }
   const int64_t total = a.rows * a.width;
   const bool packed = (a.y_stride == a.width || a.rows == 1) && uint64_t(y) % 16 == 0;
-  auto* kernel = packed ? (a.by_row ? any_rows_kernel<T, Number, V, true, true>
-                                    : any_rows_kernel<T, Number, V, false, true>)
-                        : (a.by_row ? any_rows_kernel<T, Number, V, true, false>
-                                    : any_rows_kernel<T, Number, V, false, false>);
+  auto* kernel = packed ? (a.by_row ? any_rows_kernel<T, Division, V, true, true>
+                                    : any_rows_kernel<T, Division, V, false, true>)
+                        : (a.by_row ? any_rows_kernel<T, Division, V, true, false>
+                                    : any_rows_kernel<T, Division, V, false, false>);
   kernel<<<grid_of(total, V * kThreads), kThreads, 0, a.stream>>>(
-      Number(total), Number(a.width), x, a.x_stride, y, a.y_stride, a.factor, a.mask);
+      Number(total), Division(a.width), x, a.x_stride, y, a.y_stride, a.factor, a.mask);
   return cudaGetLastError();
 }
 
@@ -195,15 +201,16 @@ cudaError_t launch(const Call& a) {
   const bool based = (uint64_t(a.x) | uint64_t(a.y)) % 16 == 0;
   // Rows of one element are decided one by one either way.
   if (packed && based && (!a.by_row || a.width == 1)) {
-    packed_kernel<T, V, U><<<grid_of(n, int64_t(U) * V * kThreads), kThreads, 0, a.stream>>>(
+    auto* kernel = n < (int64_t(1) << 34) ? packed_kernel<T, uint32_t, V, U>
+                                          : packed_kernel<T, uint64_t, V, U>;
+    kernel<<<grid_of(n, int64_t(U) * V * kThreads), kThreads, 0, a.stream>>>(
         n, static_cast<const T*>(a.x), static_cast<T*>(a.y), a.factor, a.mask);
     return cudaGetLastError();
   }
   const bool aligned =
       based && a.width % V == 0 && (a.rows == 1 || (a.x_stride % V == 0 && a.y_stride % V == 0));
-  // Divisions of 32-bit numbers while every element number fits one.
-  return n < (int64_t(1) << 32) - 2 * V * kThreads ? launch_rows<T, uint32_t>(a, aligned)
-                                                   : launch_rows<T, int64_t>(a, aligned);
+  return Narrow::fits(n + 2 * V * kThreads) ? launch_rows<T, Narrow>(a, aligned)
+                                            : launch_rows<T, Wide>(a, aligned);
 }
 
 }  // namespace

@@ -31,11 +31,38 @@ struct alignas(sizeof(T) * V) Vec {
   T v[V];
 };
 
-// Largest power of two (16 at most) that divides every value given.
+// Largest power of two (16 at most) that divides the value (of several: their
+// bitwise or).
 inline int common_bytes(uint64_t a) {
   int b = 16;
   while (b > 1 && a % b) b /= 2;
   return b;
 }
+
+// Quotient and remainder by a number that the host knows (Granlund and
+// Montgomery, "Division by invariant integers using multiplication", PLDI'94):
+// a high product, a sum and a shift for dividends below 2^31 (Narrow), the
+// division itself for larger ones (Wide).
+struct Narrow {
+  using Number = uint32_t;
+  uint32_t divisor, factor, shift;
+
+  explicit Narrow(int64_t d) : divisor(uint32_t(d)), shift(0) {
+    while ((uint64_t(1) << shift) < uint64_t(d)) ++shift;
+    factor = uint32_t(((uint64_t(1) << 32) * ((uint64_t(1) << shift) - uint64_t(d))) / uint64_t(d) + 1);
+  }
+  __device__ __forceinline__ uint32_t quotient(uint32_t n) const {
+    return (__umulhi(n, factor) + n) >> shift;
+  }
+  static bool fits(int64_t most) { return most < (int64_t(1) << 31); }
+};
+
+struct Wide {
+  using Number = int64_t;
+  int64_t divisor;
+
+  explicit Wide(int64_t d) : divisor(d) {}
+  __device__ __forceinline__ int64_t quotient(int64_t n) const { return n / divisor; }
+};
 
 }  // namespace clad3dgs

@@ -43,85 +43,93 @@ using tokens::Index;
 
 constexpr int kThreads = 256;
 
-// A lookup moves rows through registers: bound by writing the output, the index
-// and the table's rows (small ones stay in L2) come on top. Groups of lanes take
-// a row each, C vectors of 16 bytes a lane; a thread asks for the rows of U
-// tokens before it stores the first, so that four to six loads are in flight.
-template <class T, int V, int C, int U, bool kDrop>
+// A lookup is bound by writing its output (the index and the table's rows come on
+// top; small tables stay in L2). Threads take consecutive vectors of 16 bytes of
+// the output, whatever rows they belong to, so that stores are whole lines, U of
+// them each, all asked for before the first is stored.
+template <class T, class Division, int V, int U, bool kDrop>
 __global__ void __launch_bounds__(kThreads)
-    lookup_kernel(int64_t n, int64_t width, int lanes, int64_t slices,
+    lookup_kernel(typename Division::Number total, const Division vectors,
                   const T* __restrict__ table, int64_t table_stride, Index index, float factor,
-                  CounterMask mask, T* __restrict__ out) {
+                  const __grid_constant__ CounterMask mask, T* __restrict__ out) {
+  using Number = typename Division::Number;
   const unsigned long long offset = kDrop ? mask_offset(mask) : 0;
-  const int64_t block = blockIdx.x / slices;
-  const int lane = threadIdx.x % lanes, groups = kThreads / lanes;
-  const int apart = lanes * V;
-  const int64_t column = (blockIdx.x - block * slices) * (apart * C) + lane * V;
-  const int64_t first = block * (groups * U) + threadIdx.x / lanes;
+  const Number first = Number(blockIdx.x) * (U * kThreads) + threadIdx.x;
   int64_t raw[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u)
-    raw[u] = first + u * groups < n ? tokens::raw_index(index, first + u * groups) : 0;
-  Vec<T, V> v[U][C];
-  uint32_t row[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u)
-    row[u] = first + u * groups < n ? tokens::row_of(index, raw[u]) : uint32_t(index.rows);
-#pragma unroll
-  for (int u = 0; u < U; ++u)
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      v[u][c] = {};
-      if (row[u] < index.rows && column + c * apart < width)
-        v[u][c] = *reinterpret_cast<const Vec<T, V>*>(table + row[u] * table_stride + column +
-                                                      c * apart);
-    }
+  Number column[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int64_t i = first + u * groups;
-    if (i >= n) return;
+    const Number at = first + u * kThreads;
+    const Number i = vectors.quotient(at);
+    column[u] = (at - i * vectors.divisor) * V;
+    raw[u] = at < total ? tokens::raw_index(index, i) : 0;
+  }
+  Vec<T, V> v[U];
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      const int64_t at = i * width + column + c * apart;
-      if (column + c * apart >= width) break;
-      bool keep[V];
-      if (kDrop) mask_vector<V>(mask, offset, at, keep);
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-        v[u][c].v[j] = from_float<T>(!kDrop || keep[j] ? to_float(v[u][c].v[j]) * factor : 0.f);
-      if (row[u] >= index.rows) v[u][c] = {};
-      *reinterpret_cast<Vec<T, V>*>(out + at) = v[u][c];
+  for (int u = 0; u < U; ++u) {
+    v[u] = {};
+    if (first + u * kThreads < total) {
+      const uint32_t row = tokens::row_of(index, raw[u]);
+      if (row < index.rows)
+        v[u] = *reinterpret_cast<const Vec<T, V>*>(table + row * table_stride + column[u]);
     }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const Number at = first + u * kThreads;
+    if (at >= total) return;
+    bool keep[V];
+    if (kDrop) mask_vector<V, Number>(mask, offset, uint64_t(at) * V, keep);
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      v[u].v[j] = from_float<T>(!kDrop || keep[j] ? to_float(v[u].v[j]) * factor : 0.f);
+    *reinterpret_cast<Vec<T, V>*>(out + int64_t(at) * V) = v[u];
   }
 }
 
-// Rows that do not start on 16 bytes: a thread fills V consecutive elements of
-// the output, whatever rows they belong to, from single loads (adjacent
-// threads read adjacent elements, which the L1 cache gathers).
-template <class T, class Number, int V, bool kDrop>
+// Rows that do not start on 16 bytes: V consecutive elements of the output a
+// thread from single loads (neighbours hit the same lines). A vector touches
+// two rows at most, or any number of rows shorter than itself (kShort).
+template <class T, class Division, int V, bool kShort, bool kDrop>
 __global__ void __launch_bounds__(kThreads)
-    lookup_flat_kernel(Number total, Number width, const T* __restrict__ table,
-                       int64_t table_stride, Index index, float factor, CounterMask mask,
-                       T* __restrict__ out) {
+    lookup_odd_kernel(typename Division::Number total, const Division width,
+                      const T* __restrict__ table, int64_t table_stride, Index index,
+                      float factor, const __grid_constant__ CounterMask mask,
+                      T* __restrict__ out) {
+  using Number = typename Division::Number;
   const unsigned long long offset = kDrop ? mask_offset(mask) : 0;
   const Number at = (Number(blockIdx.x) * kThreads + threadIdx.x) * V;
   if (at >= total) return;
-  Number i = at / width, column = at - i * width;
-  uint32_t row = tokens::row_of(index, tokens::raw_index(index, i));
+  Number i = width.quotient(at), column = at - i * width.divisor;
   Vec<T, V> v{};
+  uint32_t row = tokens::row_of(index, tokens::raw_index(index, i));
+  if constexpr (kShort) {
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    if (at + j < total) {
-      if (column == width) {
-        column = 0;
-        row = tokens::row_of(index, tokens::raw_index(index, ++i));
+    for (int j = 0; j < V; ++j) {
+      if (at + j < total) {
+        if (column == width.divisor) {
+          column = 0;
+          row = tokens::row_of(index, tokens::raw_index(index, ++i));
+        }
+        if (row < index.rows) v.v[j] = table[row * table_stride + column];
+        ++column;
       }
-      if (row < index.rows) v.v[j] = table[row * table_stride + column];
-      ++column;
     }
+  } else {
+    // Elements before `border` from this row, the others from the next.
+    const int border = width.divisor - column < V ? int(width.divisor - column) : V;
+    const int count = total - at < V ? int(total - at) : V;
+    uint32_t next = uint32_t(index.rows);
+    if (border < count) next = tokens::row_of(index, tokens::raw_index(index, i + 1));
+    const T* here = table + row * table_stride + column;
+    const T* there = table + next * table_stride - border;
+    const int from = row < index.rows ? 0 : border, to = next < index.rows ? count : border;
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (j >= from && j < to && j < count) v.v[j] = (j < border ? here : there)[j];
   }
   bool keep[V];
-  if (kDrop) mask_vector<V>(mask, offset, at, keep);
+  if (kDrop) mask_vector<V, Number>(mask, offset, uint64_t(at), keep);
 #pragma unroll
   for (int j = 0; j < V; ++j)
     v.v[j] = from_float<T>(!kDrop || keep[j] ? to_float(v.v[j]) * factor : 0.f);
@@ -145,47 +153,45 @@ struct Lookup {
   cudaStream_t stream;
 };
 
-template <class T, int V, int C, int U>
-cudaError_t run_rows(const Lookup& a) {
-  int64_t padded;
-  const int lanes = sums::lanes_of(a.width / V, C, &padded);
-  const int64_t slices = padded / (lanes * C), tokens = kThreads / lanes * U;
-  const unsigned grid = unsigned((a.n + tokens - 1) / tokens * slices);
-  auto* kernel = a.drop ? lookup_kernel<T, V, C, U, true> : lookup_kernel<T, V, C, U, false>;
-  kernel<<<grid, kThreads, 0, a.stream>>>(a.n, a.width, lanes, slices,
-                                          static_cast<const T*>(a.table), a.stride, a.index,
-                                          a.factor, a.mask, static_cast<T*>(a.out));
-  return cudaGetLastError();
-}
+unsigned grid_of(int64_t work, int64_t each) { return unsigned((work + each - 1) / each); }
 
-template <class T, class Number, int V>
-cudaError_t run_flat(const Lookup& a) {
+template <class T, class Division>
+cudaError_t run_lookup(const Lookup& a, bool aligned) {
+  using Number = typename Division::Number;
+  constexpr int V = 16 / sizeof(T), U = 4;
+  const T* table = static_cast<const T*>(a.table);
+  T* out = static_cast<T*>(a.out);
+  if (aligned) {
+    const int64_t vectors = a.width / V, total = a.n * vectors;
+    auto* kernel =
+        a.drop ? lookup_kernel<T, Division, V, U, true> : lookup_kernel<T, Division, V, U, false>;
+    kernel<<<grid_of(total, U * kThreads), kThreads, 0, a.stream>>>(
+        Number(total), Division(vectors), table, a.stride, a.index, a.factor, a.mask, out);
+    return cudaGetLastError();
+  }
   const int64_t total = a.n * a.width;
-  const unsigned grid = unsigned((total + kThreads * V - 1) / (kThreads * V));
-  auto* kernel =
-      a.drop ? lookup_flat_kernel<T, Number, V, true> : lookup_flat_kernel<T, Number, V, false>;
-  kernel<<<grid, kThreads, 0, a.stream>>>(Number(total), Number(a.width),
-                                          static_cast<const T*>(a.table), a.stride, a.index,
-                                          a.factor, a.mask, static_cast<T*>(a.out));
-  return cudaGetLastError();
+  auto go = [&](auto* kernel, int each) {
+    kernel<<<grid_of(total, int64_t(each) * kThreads), kThreads, 0, a.stream>>>(
+        Number(total), Division(a.width), table, a.stride, a.index, a.factor, a.mask, out);
+    return cudaGetLastError();
+  };
+  if (uint64_t(out) % 16)
+    return a.drop ? go(lookup_odd_kernel<T, Division, 1, true, true>, 1)
+                  : go(lookup_odd_kernel<T, Division, 1, true, false>, 1);
+  if (a.width < V)
+    return a.drop ? go(lookup_odd_kernel<T, Division, V, true, true>, V)
+                  : go(lookup_odd_kernel<T, Division, V, true, false>, V);
+  return a.drop ? go(lookup_odd_kernel<T, Division, V, false, true>, V)
+                : go(lookup_odd_kernel<T, Division, V, false, false>, V);
 }
 
 template <class T>
-cudaError_t run_lookup(const Lookup& a) {
-  constexpr int V = 16 / sizeof(T);
-  const int bytes = common_bytes(uint64_t(a.width * sizeof(T)) | uint64_t(a.stride * sizeof(T)) |
-                                 uint64_t(a.table) | uint64_t(a.out));
-  if (bytes >= 16) {
-    switch (sums::vectors_of_lane(a.n, a.width, V)) {
-      case 4: return run_rows<T, V, 4, 1>(a);
-      case 3: return run_rows<T, V, 3, 2>(a);
-      default: return run_rows<T, V, 1, 4>(a);
-    }
-  }
-  if (uint64_t(a.out) % 16) return run_flat<T, int64_t, 1>(a);
-  // Divisions of 32-bit numbers while every element number fits one.
-  return a.n * a.width < (int64_t(1) << 32) - kThreads * V ? run_flat<T, uint32_t, V>(a)
-                                                           : run_flat<T, int64_t, V>(a);
+cudaError_t pick_lookup(const Lookup& a) {
+  const bool aligned =
+      common_bytes(uint64_t(a.width * sizeof(T)) | uint64_t(a.stride * sizeof(T)) |
+                   uint64_t(a.table) | uint64_t(a.out)) == 16;
+  return Narrow::fits(a.n * a.width + 16 * kThreads) ? run_lookup<T, Narrow>(a, aligned)
+                                                     : run_lookup<T, Wide>(a, aligned);
 }
 
 int refuse(const char* what, const char* why) {
@@ -231,12 +237,12 @@ sums::Args<T> sums_of(int64_t n, int64_t rows, int64_t width, const void* grad, 
   return a;
 }
 
-const char* sums_problem(int64_t n, int64_t rows, int64_t width, const void* grad,
-                         int64_t stride, const uint32_t* order, const void* workspace,
-                         size_t bytes) {
+const char* sums_problem(int64_t n, int64_t width, const void* grad, int64_t stride,
+                         const uint32_t* order, const void* workspace, size_t bytes,
+                         size_t need) {
   if (n > 0 && width > 0 && (!grad || !order || !workspace)) return "null array";
   if (stride < 0) return "bad row stride";
-  if (n > 0 && bytes < sums::workspace_bytes(n, width)) return "workspace too small";
+  if (bytes < need) return "workspace too small";
   if (uint64_t(workspace) % 16 || uint64_t(order) % 8) return "unaligned workspace or order";
   return nullptr;
 }
@@ -285,14 +291,15 @@ extern "C" int clad3dgs_embedding_lookup(int type, int64_t n, int64_t rows, int6
   const Lookup a{n, width, table, table_stride, x, factor_of(scale, p),
                  counter_mask(p, seed, offset, reinterpret_cast<const long long*>(offset_device)),
                  p > 0.0, out, stream};
-  return status(what, type == CLAD3DGS_F32   ? run_lookup<float>(a)
-                      : type == CLAD3DGS_F16 ? run_lookup<__half>(a)
-                                             : run_lookup<__nv_bfloat16>(a));
+  return status(what, type == CLAD3DGS_F32   ? pick_lookup<float>(a)
+                      : type == CLAD3DGS_F16 ? pick_lookup<__half>(a)
+                                             : pick_lookup<__nv_bfloat16>(a));
 }
 
-extern "C" size_t clad3dgs_embedding_workspace(int64_t n, int64_t width) {
-  if (n <= 0 || width <= 0 || n > kMostTokens || n > (int64_t(1) << 60) / width) return 0;
-  return sums::workspace_bytes(n, width);
+extern "C" size_t clad3dgs_embedding_workspace(int64_t n, int64_t rows, int64_t width,
+                                               int consume) {
+  if (n <= 0 || problem(n, rows, width, CLAD3DGS_F32, 1.0, 0.0)) return 0;
+  return consume ? sums::consume_bytes(n, rows, width) : sums::gradient_bytes(n, width);
 }
 
 extern "C" int clad3dgs_embedding_gradient(int type, int64_t n, int64_t rows, int64_t width,
@@ -305,19 +312,15 @@ extern "C" int clad3dgs_embedding_gradient(int type, int64_t n, int64_t rows, in
   const char* what = "embedding gradient";
   if (const char* why = problem(n, rows, width, type, scale, p)) return refuse(what, why);
   if (rows == 0 || width == 0) return CLAD3DGS_OK;
-  if (const char* why = sums_problem(n, rows, width, grad, grad_stride, order, workspace,
-                                     workspace_bytes))
+  if (const char* why = sums_problem(n, width, grad, grad_stride, order, workspace,
+                                     workspace_bytes, sums::gradient_bytes(n, width)))
     return refuse(what, why);
   if (!out) return refuse(what, "null array");
   auto go = [&](auto zero) {
     using T = decltype(zero);
-    const uint64_t row = uint64_t(width * sizeof(T));
-    const int bytes =
-        common_bytes(row | uint64_t(grad_stride * sizeof(T)) | uint64_t(grad));
-    return sums::run<T, T>(sums_of<T>(n, rows, width, grad, grad_stride, order, scale, p, seed,
-                                      offset, offset_device, workspace),
-                           sums::Store<T>{static_cast<T*>(out)}, bytes,
-                           common_bytes(row | uint64_t(out)), p > 0.0, stream);
+    return sums::gradient(sums_of<T>(n, rows, width, grad, grad_stride, order, scale, p, seed,
+                                     offset, offset_device, workspace),
+                          static_cast<T*>(out), p > 0.0, stream);
   };
   return status(what, type == CLAD3DGS_F32   ? go(float())
                       : type == CLAD3DGS_F16 ? go(__half())
@@ -335,22 +338,17 @@ extern "C" int clad3dgs_embedding_consume_torch_adam(
         config.bias2_sqrt > 0.f && config.bias2_sqrt <= 1.f))
     return refuse(what, "invalid Adam configuration");
   if (rows == 0 || width == 0) return CLAD3DGS_OK;
-  if (const char* why = sums_problem(n, rows, width, grad, grad_stride, order, workspace,
-                                     workspace_bytes))
+  if (const char* why = sums_problem(n, width, grad, grad_stride, order, workspace,
+                                     workspace_bytes, sums::consume_bytes(n, rows, width)))
     return refuse(what, why);
   if (!table || !first || !second) return refuse(what, "null array");
   const sums::Adam adam{table, first, second, float(rate / double(config.bias1)),
-                  1.0 / double(config.bias2_sqrt)};
+                        1.0 / double(config.bias2_sqrt)};
   auto go = [&](auto zero) {
     using T = decltype(zero);
-    const int bytes = common_bytes(uint64_t(width * sizeof(T)) |
-                                   uint64_t(grad_stride * sizeof(T)) | uint64_t(grad));
-    return sums::run<T, float>(sums_of<T>(n, rows, width, grad, grad_stride, order, scale, p,
-                                          seed, offset, offset_device, workspace),
-                               adam, bytes,
-                               common_bytes(uint64_t(width * sizeof(float)) | uint64_t(table) |
-                                            uint64_t(first) | uint64_t(second)),
-                               p > 0.0, stream);
+    return sums::consume(sums_of<T>(n, rows, width, grad, grad_stride, order, scale, p, seed,
+                                    offset, offset_device, workspace),
+                         adam, p > 0.0, stream);
   };
   return status(what, type == CLAD3DGS_F32   ? go(float())
                       : type == CLAD3DGS_F16 ? go(__half())

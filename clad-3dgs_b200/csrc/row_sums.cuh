@@ -1,7 +1,7 @@
 // Sums of gradient rows by sorted token: every table row's terms added up in
-// the order of their positions and handed, finished, to an epilogue (a store,
-// or Adam). No float atomics: the order of the additions depends on the sizes
-// alone.
+// the order of their positions. A row's sum is stored as the table's gradient,
+// or kept for the Adam pass. No float atomics: the order of the additions
+// depends on the sizes alone.
 //
 // The sorted list is cut into blocks of equal length and these into groups of
 // lanes; a group walks its tokens with the running sum of the current row in
@@ -11,12 +11,16 @@
 // partial sums in the workspace by a second kernel. Rows that no token names
 // are written by further blocks of the same launch.
 //
-// Bound by reading the gradient rows, which lie anywhere: every lane holds up to
-// C vectors of 16 bytes of a row and keeps kStages - 1 rows in flight as
-// asynchronous copies into slots of its own (60 to 80 KB an SM, twice what covers
-// the latency of memory), so the loop over tokens is rolled and the epilogue is
-// compiled once. Several vectors a lane share the loop's instructions, which
-// else cost as much time as the memory does.
+// Bound by reading the gradient rows, which lie anywhere. Every lane holds C
+// vectors of 16 bytes of a row and asks for U rows before it adds the first
+// (64 to 128 bytes a thread, 50 to 100 KB an SM in flight). Several vectors a
+// lane share the loop's instructions, which else cost as much time as the
+// memory does.
+//
+// Adam is a pass of its own over the table, because an update inside the walk
+// would wait for three loads at the end of every row (a walk over 8192 short
+// rows took 77 us instead of 52). Only the sums of rows that tokens name go
+// through memory in between, from a compact list.
 #pragma once
 #include <cuda_runtime.h>
 
@@ -32,13 +36,13 @@ namespace sums {
 
 constexpr int kThreads = 256;
 constexpr int kSms = 148;
-constexpr int kSharedPerSm = 220 * 1024;
 constexpr int kMostTokens = 2560;  // of a block: their order entries lie in shared memory
 constexpr int kLeastTokens = 8;    // of a group: keeps the joins few
 constexpr uint32_t kNoRow = ~0u;
 
-// Rows in flight per lane, and one that is being added.
-constexpr int stages_of(int c) { return c == 1 ? 6 : 3; }
+// Rows a thread asks for at once, and the blocks that an SM's registers hold.
+constexpr int rows_at_once(int c) { return c == 1 ? 4 : 2; }
+constexpr int blocks_per_sm(int elements) { return elements <= 4 ? 4 : 3; }
 
 // How [n][width] gradients are cut: C vectors of `lanes` lanes in a group,
 // `slices` groups a row, `tokens` of one group, `block` of one block.
@@ -46,14 +50,6 @@ struct Cut {
   int lanes, tokens, block;
   int64_t slices, blocks;
 };
-
-inline size_t order_bytes(int block) { return (size_t(block + 2) * sizeof(uint2) + 15) / 16 * 16; }
-
-// Shared memory of sum_kernel besides the order entries: heads, slots, kinds.
-template <class T, int V, int C>
-constexpr size_t lane_bytes() {
-  return size_t(kThreads) * (C * V * (sizeof(float) + stages_of(C) * sizeof(T)) + 1);
-}
 
 // Lanes of a group for rows of `vectors` vectors, C a lane: a short row whole;
 // else the width from 4 lanes (which read 64 bytes side by side) to 32 that
@@ -71,7 +67,7 @@ inline int lanes_of(int64_t vectors, int c, int64_t* padded) {
   return best;
 }
 
-inline Cut cut_of(int64_t n, int64_t width, int vec, int c, size_t per_block) {
+inline Cut cut_of(int64_t n, int64_t width, int vec, int c) {
   const int64_t vectors = (width + vec - 1) / vec;
   Cut cut{};
   int64_t padded;
@@ -79,9 +75,8 @@ inline Cut cut_of(int64_t n, int64_t width, int vec, int c, size_t per_block) {
   cut.slices = padded / (cut.lanes * c);
   // Tokens of a group: as many as fill the GPU in whole waves.
   const int groups = kThreads / cut.lanes;
-  const int64_t resident = std::max<int64_t>(
-      1, int64_t(kSms) * (kSharedPerSm / (per_block + order_bytes(kMostTokens))) * groups /
-             cut.slices);
+  const int64_t resident =
+      std::max<int64_t>(1, int64_t(kSms) * blocks_per_sm(c * vec) * groups / cut.slices);
   const int most = std::max(kLeastTokens, kMostTokens / groups);
   const int64_t waves = (n + resident * most - 1) / (resident * most);
   cut.tokens = int(std::max<int64_t>(kLeastTokens, (n + resident * waves - 1) / (resident * waves)));
@@ -103,14 +98,16 @@ struct Args {
   int64_t rest;    // blocks in front that write the rows without tokens
 };
 
-// ---- epilogues: element `at` of the table and V finished sums ----
+// ---- what becomes of a finished row: where it goes, and V of its sums ----
 
 template <class T>
-struct Store {
+struct Store {  // out[rows][width]
+  static constexpr bool kRest = true;  // the other rows are zeroed
   T* out;
 
+  __device__ __forceinline__ int64_t place(uint32_t row, int64_t, int64_t) const { return row; }
   template <int V>
-  __device__ __forceinline__ void operator()(int64_t at, const float (&sum)[V]) const {
+  __device__ __forceinline__ void put(int64_t at, const float (&sum)[V]) const {
     Vec<T, V> v;
 #pragma unroll
     for (int j = 0; j < V; ++j) v.v[j] = from_float<T>(sum[j]);
@@ -118,27 +115,23 @@ struct Store {
   }
 };
 
-struct Adam {
-  float *table, *first, *second;
-  float step;
-  double inv_bias2;
+template <int V>
+__device__ __forceinline__ void put(float* to, const float (&sum)[V]);
 
+struct Keep {  // sums[slot][width]; slots[row] = slot + 1
+  static constexpr bool kRest = false;
+  float* sums;
+  int32_t* slots;
+  bool by_row;  // a slot for each row, else for each token
+
+  __device__ __forceinline__ int64_t place(uint32_t row, int64_t token, int64_t column) const {
+    const int64_t slot = by_row ? int64_t(row) : token;
+    if (column == 0) slots[row] = int32_t(slot + 1);
+    return slot;
+  }
   template <int V>
-  __device__ __forceinline__ void operator()(int64_t at, const float (&sum)[V]) const {
-    constexpr int W = V < 4 ? V : 4;
-#pragma unroll
-    for (int h = 0; h < V; h += W) {
-      auto* p = reinterpret_cast<Vec<float, W>*>(table + at + h);
-      auto* m = reinterpret_cast<Vec<float, W>*>(first + at + h);
-      auto* v = reinterpret_cast<Vec<float, W>*>(second + at + h);
-      Vec<float, W> pv = *p, mv = *m, vv = *v;
-#pragma unroll
-      for (int j = 0; j < W; ++j)
-        torch_adam(pv.v[j], mv.v[j], vv.v[j], sum[h + j], step, inv_bias2);
-      *p = pv;
-      *m = mv;
-      *v = vv;
-    }
+  __device__ __forceinline__ void put(int64_t at, const float (&sum)[V]) const {
+    sums::put<V>(sums + at, sum);
   }
 };
 
@@ -173,22 +166,25 @@ __device__ __forceinline__ void clear(float (&sum)[V]) {
   for (int j = 0; j < V; ++j) sum[j] = 0.f;
 }
 
-template <int V, class End>
-__device__ __forceinline__ void finish(const End& end, int64_t at, float (&sum)[V],
-                                       float factor) {
+template <int V>
+__device__ __forceinline__ void scale(float (&sum)[V], float factor) {
 #pragma unroll
   for (int j = 0; j < V; ++j) sum[j] *= factor;
-  end.template operator()<V>(at, sum);
 }
 
-template <int kBytes>
-__device__ __forceinline__ void copy_async(void* to, const void* from) {
-  const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(to));
+// A vector that is read once.
+template <class T, int V>
+__device__ __forceinline__ Vec<T, V> read_once(const T* from) {
+  Vec<T, V> v;
+  constexpr int kBytes = V * sizeof(T);
+  static_assert(kBytes == 16 || kBytes == 4 || kBytes == 2, "vectors of 16 bytes, or one element");
   if constexpr (kBytes == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
+    *reinterpret_cast<uint4*>(&v) = __ldcs(reinterpret_cast<const uint4*>(from));
+  else if constexpr (kBytes == 4)
+    *reinterpret_cast<unsigned*>(&v) = __ldcs(reinterpret_cast<const unsigned*>(from));
   else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(at), "l"(from), "n"(kBytes)
-                 : "memory");
+    *reinterpret_cast<unsigned short*>(&v) = __ldcs(reinterpret_cast<const unsigned short*>(from));
+  return v;
 }
 
 // Rows that no token names: a gradient of zero. One warp takes 32 rows and one
@@ -217,7 +213,7 @@ __device__ void write_rest(int64_t n, int64_t rows, int64_t width, const uint2* 
   if (column >= width) return;
   const float zero[V] = {};
   while (left) {
-    end.template operator()<V>((first + __ffs(left) - 1) * width + column, zero);
+    end.template put<V>((first + __ffs(left) - 1) * width + column, zero);
     left &= left - 1;
   }
 }
@@ -233,21 +229,17 @@ enum Head : unsigned char { kNone = 0, kEnded = 1, kOpen = 2 };
 // V: elements of a vector of gradients, C: vectors of a lane, R: elements of a
 // vector of the rows without tokens.
 template <class T, int V, int C, int R, bool kDrop, class End>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, blocks_per_sm(C * V))
     sum_kernel(const __grid_constant__ Args<T> a, const End end) {
-  if (blockIdx.x < a.rest) {
-    write_rest<R, End>(a.n, a.rows, a.width, a.order, end);
-    return;
+  if constexpr (End::kRest) {
+    if (blockIdx.x < a.rest) {
+      write_rest<R, End>(a.n, a.rows, a.width, a.order, end);
+      return;
+    }
   }
-  constexpr int kBytes = V * sizeof(T);
-  constexpr int kStages = stages_of(C);
-  extern __shared__ __align__(16) char shared[];
-  uint2* entries = reinterpret_cast<uint2*>(shared);
-  const size_t order_size = (size_t(a.cut.block + 2) * sizeof(uint2) + 15) / 16 * 16;
-  float* heads = reinterpret_cast<float*>(shared + order_size);  // [C][kThreads][V]
-  char* slots = shared + order_size + size_t(kThreads) * C * V * sizeof(float);
-  unsigned char* kinds =
-      reinterpret_cast<unsigned char*>(slots + size_t(kThreads) * kStages * C * kBytes);
+  __shared__ uint2 entries[kMostTokens + 2];
+  __shared__ __align__(16) float heads[C * kThreads * V];
+  __shared__ unsigned char kinds[kThreads];
 
   const unsigned long long offset = kDrop ? mask_offset(a.mask) : 0;
   const int64_t job = blockIdx.x - a.rest;
@@ -287,10 +279,14 @@ __global__ void __launch_bounds__(kThreads)
     for (int c = 0; c < C; ++c) clear<V>(sum[c]);
   };
   uint32_t row = begin < stop ? entry[begin].x : kNoRow;
-  auto done = [&] {
+  auto done = [&](int i) {  // i: a token of the row
+    const int64_t at = end.place(row, first + i, column) * a.width + column;
 #pragma unroll
     for (int c = 0; c < C; ++c)
-      if (live[c]) finish<V>(end, row * a.width + column + c * apart, sum[c], a.factor);
+      if (live[c]) {
+        scale<V>(sum[c], a.factor);
+        end.template put<V>(at + c * apart, sum[c]);
+      }
   };
   auto put_head = [&] {
 #pragma unroll
@@ -300,81 +296,53 @@ __global__ void __launch_bounds__(kThreads)
   bool before = begin < stop && entry[begin - 1].x == row;
   Head kind = kNone;
 
-  // One token's terms; hands the row before on when a new one begins.
-  auto take = [&](const uint2& token, const Vec<T, V> (&g)[C]) {
-    if (token.x != row) {
-      if (before) {
-        put_head();
-        kind = kEnded;
-        before = false;
-      } else {
-        done();
-      }
-      row = token.x;
-      reset();
-    }
+  auto add_terms = [&](uint32_t position, const Vec<T, V> (&g)[C]) {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      if constexpr (kDrop) {
-        bool keep[V];
-        mask_vector<V>(a.mask, offset, token.y * a.width + column + c * apart, keep);
+      bool keep[V];
+      if constexpr (kDrop)
+        mask_vector<V>(a.mask, offset, uint64_t(position * a.width + column + c * apart), keep);
 #pragma unroll
-        for (int j = 0; j < V; ++j) sum[c][j] += keep[j] ? to_float(g[c].v[j]) : 0.f;
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) sum[c][j] += to_float(g[c].v[j]);
-      }
+      for (int j = 0; j < V; ++j)
+        sum[c][j] += !kDrop || keep[j] ? to_float(g[c].v[j]) : 0.f;
     }
   };
 
   const T* grad = a.grad + column;
-  if constexpr (kBytes >= 4) {
-    char* mine = slots + threadIdx.x * kBytes;
-    constexpr int kStageBytes = kThreads * C * kBytes;
-    auto fetch = [&](int i, int slot) {
-      if (i < stop) {
-        const T* from = grad + entry[i].y * a.stride;
+  constexpr int U = rows_at_once(C);
+  for (int i = begin; i < stop; i += U) {
+    uint2 token[U];
+    Vec<T, V> g[U][C];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i + u < stop) {
+        token[u] = entry[i + u];
+        const T* from = grad + token[u].y * a.stride;
 #pragma unroll
         for (int c = 0; c < C; ++c)
-          if (live[c])
-            copy_async<kBytes>(mine + slot * kStageBytes + c * (kThreads * kBytes),
-                               from + c * apart);
+          if (live[c]) g[u][c] = read_once<T, V>(from + c * apart);
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    };
+    if (i + U <= stop && token[U - 1].x == row) {  // all of one row, which is the current one
 #pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) fetch(begin + s, s);
-    int slot = 0;
-    for (int i = begin; i < stop; ++i) {
-      fetch(i + kStages - 1, slot == 0 ? kStages - 1 : slot - 1);
-      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
-      Vec<T, V> g[C];
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-        g[c] = *reinterpret_cast<const Vec<T, V>*>(mine + slot * kStageBytes +
-                                                   c * (kThreads * kBytes));
-      take(entry[i], g);
-      if (++slot == kStages) slot = 0;
+      for (int u = 0; u < U; ++u) add_terms(token[u].y, g[u]);
+      continue;
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
-  } else {
-    // Single 16-bit elements, which no asynchronous copy takes: loads in batches.
-    constexpr int kBatch = 4;
-    for (int i = begin; i < stop; i += kBatch) {
-      Vec<T, V> g[kBatch][C];
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u)
-        if (i + u < stop) {
-#pragma unroll
-          for (int c = 0; c < C; ++c)
-            if (live[c])
-              g[u][c] = *reinterpret_cast<const Vec<T, V>*>(grad + entry[i + u].y * a.stride +
-                                                            c * apart);
+    for (int u = 0; u < U; ++u)
+      if (i + u < stop) {
+        if (token[u].x != row) {  // hand the row before on
+          if (before) {
+            put_head();
+            kind = kEnded;
+            before = false;
+          } else {
+            done(i + u - 1);
+          }
+          row = token[u].x;
+          reset();
         }
-#pragma unroll
-      for (int u = 0; u < kBatch; ++u)
-        if (i + u < stop) take(entry[i + u], g[u]);
-    }
+        add_terms(token[u].y, g[u]);
+      }
   }
 
   // The group's last row: finished, a head that stays open, or continued by
@@ -386,7 +354,7 @@ __global__ void __launch_bounds__(kThreads)
       put_head();
       kind = after ? kOpen : kEnded;
     } else if (!after) {
-      done();
+      done(stop - 1);
     }
   }
   if (lane == 0) kinds[group] = kind;
@@ -408,7 +376,7 @@ __global__ void __launch_bounds__(kThreads)
   };
   if (continued) {
     if (join(group + 1)) put_partial(2 * block + 1);
-    else done();
+    else done(stop - 1);
   }
   if (group == 0 && kind != kNone) {
     reset();
@@ -453,7 +421,8 @@ __global__ void __launch_bounds__(kThreads)
   clear<V>(sum);
   add<V>(a.partial + (2 * block + 1) * a.width + column, sum);
   for (int g = 0; g < groups; ++g) add<V>(shares + (g * lanes + lane) * V, sum);
-  finish<V>(end, row * a.width + column, sum, a.factor);
+  scale<V>(sum, a.factor);
+  end.template put<V>(end.place(row, stop - 1, column) * a.width + column, sum);
 }
 
 // The launch without any token.
@@ -463,36 +432,81 @@ __global__ void __launch_bounds__(kThreads)
   write_rest<R, End>(0, rows, width, nullptr, end);
 }
 
+// ---- Adam ----
+
+struct Adam {
+  float *table, *first, *second;
+  float step;
+  double inv_bias2;
+};
+
+// Vectors of W elements of the table, U of them a thread, all loaded before the
+// first is updated. slots null: no token at all. Bound by memory: six streams
+// of the table's size.
+template <class Division, int W, int U>
+__global__ void __launch_bounds__(kThreads)
+    adam_kernel(typename Division::Number total, const Division vectors, int64_t width,
+                const int32_t* __restrict__ slots, const float* __restrict__ sums, const Adam a) {
+  using Number = typename Division::Number;
+  using F = Vec<float, W>;
+  const Number first = Number(blockIdx.x) * (U * kThreads) + threadIdx.x;
+  F p[U], m[U], v[U], g[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const Number at = first + u * kThreads;
+    if (at < total) {
+      const Number row = vectors.quotient(at);
+      const int32_t slot = slots ? slots[row] : 0;
+      p[u] = reinterpret_cast<const F*>(a.table)[at];
+      m[u] = reinterpret_cast<const F*>(a.first)[at];
+      v[u] = reinterpret_cast<const F*>(a.second)[at];
+      g[u] = {};
+      if (slot > 0)
+        g[u] = *reinterpret_cast<const F*>(sums + int64_t(slot - 1) * width +
+                                           int64_t(at - row * vectors.divisor) * W);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const Number at = first + u * kThreads;
+    if (at >= total) return;
+#pragma unroll
+    for (int j = 0; j < W; ++j)
+      torch_adam(p[u].v[j], m[u].v[j], v[u].v[j], g[u].v[j], a.step, a.inv_bias2);
+    reinterpret_cast<F*>(a.table)[at] = p[u];
+    reinterpret_cast<F*>(a.first)[at] = m[u];
+    reinterpret_cast<F*>(a.second)[at] = v[u];
+  }
+}
+
 // ---- host ----
 
-// Vectors of a lane: one, three or four, whatever covers a row with the fewest
-// idle lanes; more of them where that is equal, unless the rows are so few
-// that the groups would not fill the GPU.
-inline int vectors_of_lane(int64_t n, int64_t width, int vec) {
+// Vectors of a lane: one, three or four floats' vectors, one or two of 16-bit
+// elements (16 running sums a lane at most), whatever covers a row with the
+// fewest idle lanes; more of them where that is equal, unless the rows are so
+// few that the groups would not fill the GPU.
+inline int vectors_of_lane(int64_t n, int64_t width, int vec, bool floats) {
   const int64_t vectors = (width + vec - 1) / vec;
-  int64_t one, three, four;
+  const int more = floats ? 4 : 2, other = floats ? 3 : 1;
+  int64_t one, some, most;
   lanes_of(vectors, 1, &one);
-  lanes_of(vectors, 3, &three);
-  lanes_of(vectors, 4, &four);
-  const int64_t least = std::min(one, std::min(three, four));
+  lanes_of(vectors, other, &some);
+  lanes_of(vectors, more, &most);
+  const int64_t least = std::min(one, std::min(some, most));
   auto fills = [&](int c, int64_t padded) {
     return padded == least && n * (padded / c) >= int64_t(kSms) * 512 * kLeastTokens;
   };
-  if (fills(4, four)) return 4;
-  return fills(3, three) ? 3 : 1;
+  if (fills(more, most)) return more;
+  return fills(other, some) ? other : 1;
 }
 
 template <class T, int V, int C, int R, class End>
 cudaError_t run_cut(Args<T> a, const End& end, bool drop, cudaStream_t stream) {
-  a.cut = cut_of(a.n, a.width, V, C, lane_bytes<T, V, C>());
-  a.rest = rest_blocks(a.rows, a.width, R);
-  const size_t shared = order_bytes(a.cut.block) + lane_bytes<T, V, C>();
+  a.cut = cut_of(a.n, a.width, V, C);
+  a.rest = End::kRest ? rest_blocks(a.rows, a.width, R) : 0;
   const unsigned grid = unsigned(a.rest + a.cut.blocks * a.cut.slices);
   auto* kernel = drop ? sum_kernel<T, V, C, R, true, End> : sum_kernel<T, V, C, R, false, End>;
-  const cudaError_t e =
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared));
-  if (e != cudaSuccess) return e;
-  kernel<<<grid, kThreads, shared, stream>>>(a, end);
+  kernel<<<grid, kThreads, 0, stream>>>(a, end);
   if (a.cut.blocks > 1) {
     int64_t padded;
     const int lanes = lanes_of((a.width + V - 1) / V, 1, &padded);
@@ -504,39 +518,91 @@ cudaError_t run_cut(Args<T> a, const End& end, bool drop, cudaStream_t stream) {
 
 template <class T, int V, int R, class End>
 cudaError_t run_sums(const Args<T>& a, const End& end, bool drop, cudaStream_t stream) {
-  switch (vectors_of_lane(a.n, a.width, V)) {
-    case 4: return run_cut<T, V, 4, R, End>(a, end, drop, stream);
-    case 3: return run_cut<T, V, 3, R, End>(a, end, drop, stream);
-    default: return run_cut<T, V, 1, R, End>(a, end, drop, stream);
-  }
+  constexpr bool kFloats = sizeof(T) == 4;
+  const int c = vectors_of_lane(a.n, a.width, V, kFloats);
+  if (c == 1) return run_cut<T, V, 1, R, End>(a, end, drop, stream);
+  if constexpr (kFloats)
+    return c == 3 ? run_cut<T, V, 3, R, End>(a, end, drop, stream)
+                  : run_cut<T, V, 4, R, End>(a, end, drop, stream);
+  else
+    return run_cut<T, V, 2, R, End>(a, end, drop, stream);
 }
 
-// `bytes`: what every row of the gradients starts on; `end_bytes`: the same of
-// the epilogue's arrays, whose elements are E. Vectors are 16 bytes where both
-// allow it, else single elements.
-template <class T, class E, class End>
-cudaError_t run(const Args<T>& a, const End& end, int bytes, int end_bytes, bool drop,
-                cudaStream_t stream) {
-  constexpr int kMost = 16 / sizeof(T), kEndMost = 16 / sizeof(E);
+template <class T>
+bool aligned(const Args<T>& a) {
+  return common_bytes(uint64_t(a.width * sizeof(T)) | uint64_t(a.stride * sizeof(T)) |
+                      uint64_t(a.grad)) == 16;
+}
+
+// Vectors are 16 bytes where the rows of all arrays begin on 16, else single
+// elements.
+template <class T>
+cudaError_t gradient(const Args<T>& a, T* out, bool drop, cudaStream_t stream) {
+  constexpr int V = 16 / sizeof(T);
+  const Store<T> end{out};
+  const bool whole = common_bytes(uint64_t(a.width * sizeof(T)) | uint64_t(out)) == 16;
   if (a.n == 0) {
-    if (end_bytes >= 16)
-      rest_kernel<kEndMost, End><<<unsigned(rest_blocks(a.rows, a.width, kEndMost)), kThreads, 0,
-                                   stream>>>(a.rows, a.width, end);
-    else
-      rest_kernel<1, End><<<unsigned(rest_blocks(a.rows, a.width, 1)), kThreads, 0, stream>>>(
-          a.rows, a.width, end);
+    auto* kernel = whole ? rest_kernel<V, Store<T>> : rest_kernel<1, Store<T>>;
+    kernel<<<unsigned(rest_blocks(a.rows, a.width, whole ? V : 1)), kThreads, 0, stream>>>(
+        a.rows, a.width, end);
     return cudaGetLastError();
   }
-  if (end_bytes < 16) return run_sums<T, 1, 1, End>(a, end, drop, stream);
-  if (bytes < 16) return run_sums<T, 1, kEndMost, End>(a, end, drop, stream);
-  return run_sums<T, kMost, kEndMost, End>(a, end, drop, stream);
+  if (!whole) return run_sums<T, 1, 1>(a, end, drop, stream);
+  return aligned(a) ? run_sums<T, V, V>(a, end, drop, stream)
+                    : run_sums<T, 1, V>(a, end, drop, stream);
 }
 
-// Workspace for any cut of these sizes: a group has kLeastTokens at least, a
-// block at least a group for each 32 lanes.
-inline size_t workspace_bytes(int64_t n, int64_t width) {
+// Workspace of the partial sums for any cut of these sizes: a group has
+// kLeastTokens at least, a block at least a group for each 32 lanes.
+inline size_t gradient_bytes(int64_t n, int64_t width) {
   const int64_t least = kThreads / 32 * kLeastTokens;
-  return size_t(2 * ((n + least - 1) / least)) * width * sizeof(float);
+  const size_t bytes = size_t(2 * ((n + least - 1) / least)) * width * sizeof(float);
+  return (bytes + 15) / 16 * 16;
+}
+
+// ... and of Adam: a slot number for each row, sums for the rows that tokens
+// name (no more than rows, nor than tokens).
+inline size_t slot_bytes(int64_t rows) { return (size_t(rows) * sizeof(int32_t) + 15) / 16 * 16; }
+
+inline size_t consume_bytes(int64_t n, int64_t rows, int64_t width) {
+  if (n == 0) return 0;
+  return gradient_bytes(n, width) + slot_bytes(rows) +
+         size_t(std::min(n, rows)) * width * sizeof(float);
+}
+
+template <class Division, int W>
+cudaError_t run_adam(int64_t rows, int64_t width, const int32_t* slots, const float* sums,
+                     const Adam& adam, cudaStream_t stream) {
+  constexpr int U = 2;
+  const int64_t vectors = width / W, total = rows * vectors;
+  adam_kernel<Division, W, U><<<unsigned((total + U * kThreads - 1) / (U * kThreads)), kThreads, 0,
+                                stream>>>(typename Division::Number(total), Division(vectors),
+                                          width, slots, sums, adam);
+  return cudaGetLastError();
+}
+
+template <class T>
+cudaError_t consume(const Args<T>& a, const Adam& adam, bool drop, cudaStream_t stream) {
+  constexpr int V = 16 / sizeof(T);
+  int32_t* slots = nullptr;
+  float* kept = nullptr;
+  if (a.n > 0) {
+    char* at = reinterpret_cast<char*>(a.partial) + gradient_bytes(a.n, a.width);
+    slots = reinterpret_cast<int32_t*>(at);
+    kept = reinterpret_cast<float*>(at + slot_bytes(a.rows));
+    cudaError_t e = cudaMemsetAsync(slots, 0, size_t(a.rows) * sizeof(int32_t), stream);
+    if (e != cudaSuccess) return e;
+    const Keep end{kept, slots, a.rows <= a.n};
+    e = aligned(a) ? run_sums<T, V, 1>(a, end, drop, stream)
+                   : run_sums<T, 1, 1>(a, end, drop, stream);
+    if (e != cudaSuccess) return e;
+  }
+  const bool whole = common_bytes(uint64_t(a.width * sizeof(float)) | uint64_t(adam.table) |
+                                  uint64_t(adam.first) | uint64_t(adam.second)) == 16;
+  const bool narrow = Narrow::fits(a.rows * a.width + 2 * kThreads);
+  auto* run = whole ? (narrow ? run_adam<Narrow, 4> : run_adam<Wide, 4>)
+                    : (narrow ? run_adam<Narrow, 1> : run_adam<Wide, 1>);
+  return run(a.rows, a.width, slots, kept, adam, stream);
 }
 
 }  // namespace sums

@@ -1,5 +1,5 @@
 """Tables whose rows many Gaussians (or tokens) share: lookup with scaling, the
-table's gradient by sorted tokens, and that gradient handed straight to Adam.
+table's gradient by sorted tokens, and that gradient handed to Adam.
 
 A codebook of SH coefficients, per-view or per-token embeddings: an index per
 token names a row of `table` [rows, width].
@@ -9,8 +9,8 @@ token names a row of `table` [rows, width].
   same pass; differentiable once in the table.
 * `lookup_gradient(grad, index, rows, ...)`: the adjoint, a dense [rows, width].
 * `consume_torch_adam(table, first, second, grad, index, ...)`: the adjoint and
-  torch-fused Adam on the table in one go, like the SH consume entries: the
-  gradient is never written.
+  torch-fused Adam on the table in one call, like the SH consume entries; of
+  the gradient only the rows that tokens name exist, in a workspace.
 * `token_order(index, rows)`: the tokens sorted by row. The two calls above sort
   for themselves unless they are given it; a program whose assignments stay
   the same over many steps sorts once.
@@ -153,7 +153,7 @@ def lookup_gradient(grad, index, rows, *, scale=1.0, padding_index=None, p=0.0, 
     if out.numel() == 0:
         return out
     lib = native.library()
-    workspace = _bytes(lib.clad3dgs_embedding_workspace(tokens, width), device)
+    workspace = _bytes(lib.clad3dgs_embedding_workspace(tokens, rows, width, 0), device)
     on_device(device, lambda: native.check(lib.clad3dgs_embedding_gradient(
         TYPES[grad.dtype], tokens, rows, width, native.ptr(grad), stride,
         native.ptr(order.pairs), scale, p, seed, number, address, out.data_ptr(),
@@ -190,7 +190,7 @@ def consume_torch_adam(table, first, second, grad, index, *, rate, bias1, bias2_
     if table.numel() == 0:
         return
     lib = native.library()
-    workspace = _bytes(lib.clad3dgs_embedding_workspace(tokens, width), device)
+    workspace = _bytes(lib.clad3dgs_embedding_workspace(tokens, rows, width, 1), device)
     on_device(device, lambda: native.check(lib.clad3dgs_embedding_consume_torch_adam(
         TYPES[grad.dtype], tokens, rows, width, native.ptr(grad), stride,
         native.ptr(order.pairs), scale, p, seed, number, address, table.data_ptr(),

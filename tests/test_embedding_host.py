@@ -99,8 +99,11 @@ def test_workspaces():
     lib = native.library()
     assert lib.clad3dgs_token_order_workspace(0, 5) == 0
     assert lib.clad3dgs_token_order_workspace(2 ** 31, 5) == 0
-    assert lib.clad3dgs_embedding_workspace(0, 5) == 0
-    assert lib.clad3dgs_embedding_workspace(5, 0) == 0
+    assert lib.clad3dgs_embedding_workspace(0, 5, 5, 0) == 0
+    assert lib.clad3dgs_embedding_workspace(5, -1, 5, 0) == 0
+    assert lib.clad3dgs_embedding_workspace(2 ** 31, 5, 5, 1) == 0
     sizes = [lib.clad3dgs_token_order_workspace(n, 4096) for n in (1, 10_000, 70_000, 1_000_000)]
     assert sizes == sorted(sizes) and sizes[2] > 0  # few tokens need none
-    assert lib.clad3dgs_embedding_workspace(1_000_000, 48) > lib.clad3dgs_embedding_workspace(10, 48)
+    few, many = (lib.clad3dgs_embedding_workspace(n, 4096, 48, 0) for n in (10, 1_000_000))
+    assert 0 < few < many
+    assert lib.clad3dgs_embedding_workspace(10, 4096, 48, 1) >= few + 4 * 4096 + 10 * 48 * 4
