@@ -8,12 +8,14 @@
 // one rounding to the element type.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <string>
 
 #include "clad3dgs_b200.h"
 #include "counter_mask.cuh"
 #include "element_types.cuh"
+#include "launch.cuh"
 
 namespace clad3dgs {
 int fail(int code, const std::string& message);  // gaussian_step.cu
@@ -22,42 +24,48 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// Bound by moving the elements once each way; the generator's ten rounds serve
-// four elements and hide behind that while every access is 16 bytes. Vectors
-// of V elements, U of them a thread, all loaded before the first is drawn for.
+// Bound by moving the elements once each way, and nearly as much by the
+// generator: twenty products of 32 x 32 bits for four elements, at a quarter of
+// the rate of other instructions. Every access is a vector of 16 bytes.
 
-// Packed rows: element numbers are addresses.
-template <class T, class Number, int V, int U>
-__global__ void __launch_bounds__(kThreads)
-    packed_kernel(int64_t n, const T* x, T* y, float factor,
+// x with the dropped elements at zero and the others times the factor.
+template <class T, int V>
+__device__ __forceinline__ Vec<T, V> drop(const Vec<T, V>& x, const bool (&keep)[V],
+                                          float factor) {
+  float f[V];
+  unpack<T, V>(x, f);
+#pragma unroll
+  for (int j = 0; j < V; ++j) f[j] = keep[j] ? f[j] * factor : 0.f;
+  return pack<T, V>(f);
+}
+
+// Packed rows: element numbers are addresses. Blocks stay and take a vector a
+// round: the first two rounds' products that hang on the offset alone are made
+// once, and with 64 warps an SM the next vectors arrive while these are drawn
+// for (16384 x 4096 bf16: 61 us, 66 with eight blocks of 256 threads, 72 to 80
+// with a block for every one, two or four vectors a thread; the words alone
+// take 37 us, the copy alone 42).
+constexpr int kStayThreads = 1024, kStayBlocks = 2;
+
+template <class T, class Number, int V>
+__global__ void __launch_bounds__(kStayThreads, kStayBlocks)
+    packed_kernel(int64_t vectors, int rest, const T* x, T* y, float factor,
                   const __grid_constant__ CounterMask mask) {
+  wait_before();
   const unsigned long long offset = mask_offset(mask);
-  const int64_t first = (int64_t(blockIdx.x) * (U * kThreads) + threadIdx.x) * V;
-  constexpr int64_t kApart = int64_t(kThreads) * V;
-  Vec<T, V> v[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int64_t at = first + u * kApart;
-    if (at + V <= n) v[u] = *reinterpret_cast<const Vec<T, V>*>(x + at);
-    else
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (at + j < n) v[u].v[j] = x[at + j];
-  }
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int64_t at = first + u * kApart;
-    if (at >= n) return;
+  const int64_t first = int64_t(blockIdx.x) * kStayThreads + threadIdx.x;
+  for (int64_t i = first; i < vectors; i += int64_t(gridDim.x) * kStayThreads) {
+    const Vec<T, V> v = reinterpret_cast<const Vec<T, V>*>(x)[i];
     bool keep[V];
-    mask_vector<V, Number>(mask, offset, at, keep);
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-      v[u].v[j] = from_float<T>(keep[j] ? to_float(v[u].v[j]) * factor : 0.f);
-    if (at + V <= n) *reinterpret_cast<Vec<T, V>*>(y + at) = v[u];
-    else
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (at + j < n) y[at + j] = v[u].v[j];
+    mask_vector<V, Number>(mask, offset, i * V, keep);
+    reinterpret_cast<Vec<T, V>*>(y)[i] = drop<T, V>(v, keep, factor);
+  }
+  if (first < rest) {  // elements behind the last vector
+    const int64_t at = vectors * V + first;
+    const uint4 words = mask_words(mask, offset, Number(at / 4));
+    const bool keep[1] = {mask.keeps(word_of(words, unsigned(at % 4)))};
+    reinterpret_cast<Vec<T, 1>*>(y)[at] =
+        drop<T, 1>(reinterpret_cast<const Vec<T, 1>*>(x)[at], keep, factor);
   }
 }
 
@@ -69,6 +77,7 @@ __global__ void __launch_bounds__(kThreads)
                         int64_t x_stride, T* y, int64_t y_stride, float factor,
                         const __grid_constant__ CounterMask mask) {
   using Number = typename Division::Number;
+  wait_before();
   const unsigned long long offset = mask_offset(mask);
   const Number first = Number(blockIdx.x) * (U * kThreads) + threadIdx.x;
   Vec<T, V> v[U];
@@ -92,9 +101,7 @@ __global__ void __launch_bounds__(kThreads)
     } else {
       mask_vector<V>(mask, offset, uint64_t(first + u * kThreads) * V, keep);
     }
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-      v[u].v[j] = from_float<T>(keep[j] ? to_float(v[u].v[j]) * factor : 0.f);
+    v[u] = drop<T, V>(v[u], keep, factor);
     *reinterpret_cast<Vec<T, V>*>(y + row[u] * y_stride + column[u]) = v[u];
   }
 }
@@ -108,6 +115,7 @@ __global__ void __launch_bounds__(kThreads)
                     int64_t x_stride, T* y, int64_t y_stride, float factor,
                     const __grid_constant__ CounterMask mask) {
   using Number = typename Division::Number;
+  wait_before();
   const unsigned long long offset = mask_offset(mask);
   const Number at = (Number(blockIdx.x) * kThreads + threadIdx.x) * V;
   if (at >= total) return;
@@ -138,9 +146,7 @@ __global__ void __launch_bounds__(kThreads)
   } else {
     mask_vector<V, Number>(mask, offset, at, keep);
   }
-#pragma unroll
-  for (int j = 0; j < V; ++j)
-    v.v[j] = from_float<T>(keep[j] ? to_float(v.v[j]) * factor : 0.f);
+  v = drop<T, V>(v, keep, factor);
   if (kPacked && at + V <= total) {
     *reinterpret_cast<Vec<T, V>*>(y + at) = v;
     return;
@@ -178,9 +184,8 @@ cudaError_t launch_rows(const Call& a, bool aligned) {
     const int64_t vectors = a.width / V, total = a.rows * vectors;
     auto* kernel = a.by_row ? aligned_rows_kernel<T, Division, V, U, true>
                             : aligned_rows_kernel<T, Division, V, U, false>;
-    kernel<<<grid_of(total, U * kThreads), kThreads, 0, a.stream>>>(
+    return launch_after(kernel, grid_of(total, U * kThreads), kThreads, 0, a.stream,
         Number(total), Division(vectors), x, a.x_stride, y, a.y_stride, a.factor, a.mask);
-    return cudaGetLastError();
   }
   const int64_t total = a.rows * a.width;
   const bool packed = (a.y_stride == a.width || a.rows == 1) && uint64_t(y) % 16 == 0;
@@ -188,24 +193,24 @@ cudaError_t launch_rows(const Call& a, bool aligned) {
                                     : any_rows_kernel<T, Division, V, false, true>)
                         : (a.by_row ? any_rows_kernel<T, Division, V, true, false>
                                     : any_rows_kernel<T, Division, V, false, false>);
-  kernel<<<grid_of(total, V * kThreads), kThreads, 0, a.stream>>>(
-      Number(total), Division(a.width), x, a.x_stride, y, a.y_stride, a.factor, a.mask);
-  return cudaGetLastError();
+  return launch_after(kernel, grid_of(total, V * kThreads), kThreads, 0, a.stream,
+        Number(total), Division(a.width), x, a.x_stride, y, a.y_stride, a.factor, a.mask);
 }
 
 template <class T>
 cudaError_t launch(const Call& a) {
-  constexpr int V = 16 / sizeof(T), U = 2;
+  constexpr int V = 16 / sizeof(T);
   const int64_t n = a.rows * a.width;
   const bool packed = a.rows == 1 || (a.x_stride == a.width && a.y_stride == a.width);
   const bool based = (uint64_t(a.x) | uint64_t(a.y)) % 16 == 0;
   // Rows of one element are decided one by one either way.
   if (packed && based && (!a.by_row || a.width == 1)) {
-    auto* kernel = n < (int64_t(1) << 34) ? packed_kernel<T, uint32_t, V, U>
-                                          : packed_kernel<T, uint64_t, V, U>;
-    kernel<<<grid_of(n, int64_t(U) * V * kThreads), kThreads, 0, a.stream>>>(
-        n, static_cast<const T*>(a.x), static_cast<T*>(a.y), a.factor, a.mask);
-    return cudaGetLastError();
+    auto* kernel =
+        n < (int64_t(1) << 34) ? packed_kernel<T, uint32_t, V> : packed_kernel<T, uint64_t, V>;
+    const unsigned blocks = std::max(1u, grid_of(n / V, kStayThreads));
+    return launch_after(kernel, std::min(blocks, 148u * kStayBlocks), kStayThreads, 0, a.stream,
+                        n / V, int(n % V), static_cast<const T*>(a.x), static_cast<T*>(a.y),
+                        a.factor, a.mask);
   }
   const bool aligned =
       based && a.width % V == 0 && (a.rows == 1 || (a.x_stride % V == 0 && a.y_stride % V == 0));

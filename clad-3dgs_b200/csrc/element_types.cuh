@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 namespace clad3dgs {
 
@@ -30,6 +31,32 @@ template <class T, int V>
 struct alignas(sizeof(T) * V) Vec {
   T v[V];
 };
+
+// A vector to floats and back, two 16-bit elements an instruction.
+template <class T, int V>
+__device__ __forceinline__ void unpack(const Vec<T, V>& from, float (&to)[V]) {
+#pragma unroll
+  for (int j = 0; j < V; ++j) to[j] = to_float(from.v[j]);
+}
+
+template <class T, int V>
+__device__ __forceinline__ Vec<T, V> pack(const float (&from)[V]) {
+  Vec<T, V> to;
+  if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+#pragma unroll
+    for (int j = 0; j < V; j += 2) {
+      if constexpr (std::is_same<T, __half>::value)
+        *reinterpret_cast<__half2*>(&to.v[j]) = __floats2half2_rn(from[j], from[j + 1]);
+      else
+        *reinterpret_cast<__nv_bfloat162*>(&to.v[j]) =
+            __floats2bfloat162_rn(from[j], from[j + 1]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) to.v[j] = from_float<T>(from[j]);
+  }
+  return to;
+}
 
 // Largest power of two (16 at most) that divides the value (of several: their
 // bitwise or).

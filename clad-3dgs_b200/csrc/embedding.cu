@@ -21,6 +21,7 @@
 #include "clad3dgs_b200.h"
 #include "counter_mask.cuh"
 #include "element_types.cuh"
+#include "launch.cuh"
 #include "row_sums.cuh"
 #include "token_order.cuh"
 
@@ -43,6 +44,17 @@ using tokens::Index;
 
 constexpr int kThreads = 256;
 
+// The output's elements: table elements times the factor, dropped ones at zero.
+template <class T, int V, bool kDrop>
+__device__ __forceinline__ Vec<T, V> finish(const Vec<T, V>& x, const bool (&keep)[V],
+                                            float factor) {
+  float f[V];
+  unpack<T, V>(x, f);
+#pragma unroll
+  for (int j = 0; j < V; ++j) f[j] = !kDrop || keep[j] ? f[j] * factor : 0.f;
+  return pack<T, V>(f);
+}
+
 // A lookup is bound by writing its output (the index and the table's rows come on
 // top; small tables stay in L2). Threads take consecutive vectors of 16 bytes of
 // the output, whatever rows they belong to, so that stores are whole lines, U of
@@ -53,6 +65,7 @@ __global__ void __launch_bounds__(kThreads)
                   const T* __restrict__ table, int64_t table_stride, Index index, float factor,
                   const __grid_constant__ CounterMask mask, T* __restrict__ out) {
   using Number = typename Division::Number;
+  wait_before();
   const unsigned long long offset = kDrop ? mask_offset(mask) : 0;
   const Number first = Number(blockIdx.x) * (U * kThreads) + threadIdx.x;
   int64_t raw[U];
@@ -80,10 +93,8 @@ __global__ void __launch_bounds__(kThreads)
     if (at >= total) return;
     bool keep[V];
     if (kDrop) mask_vector<V, Number>(mask, offset, uint64_t(at) * V, keep);
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-      v[u].v[j] = from_float<T>(!kDrop || keep[j] ? to_float(v[u].v[j]) * factor : 0.f);
-    *reinterpret_cast<Vec<T, V>*>(out + int64_t(at) * V) = v[u];
+    *reinterpret_cast<Vec<T, V>*>(out + int64_t(at) * V) =
+        finish<T, V, kDrop>(v[u], keep, factor);
   }
 }
 
@@ -97,6 +108,7 @@ __global__ void __launch_bounds__(kThreads)
                       float factor, const __grid_constant__ CounterMask mask,
                       T* __restrict__ out) {
   using Number = typename Division::Number;
+  wait_before();
   const unsigned long long offset = kDrop ? mask_offset(mask) : 0;
   const Number at = (Number(blockIdx.x) * kThreads + threadIdx.x) * V;
   if (at >= total) return;
@@ -123,16 +135,17 @@ __global__ void __launch_bounds__(kThreads)
     if (border < count) next = tokens::row_of(index, tokens::raw_index(index, i + 1));
     const T* here = table + row * table_stride + column;
     const T* there = table + next * table_stride - border;
-    const int from = row < index.rows ? 0 : border, to = next < index.rows ? count : border;
+    const int until = row < index.rows ? (border < count ? border : count) : 0;
+    const int from = next < index.rows ? border : V;
 #pragma unroll
-    for (int j = 0; j < V; ++j)
-      if (j >= from && j < to && j < count) v.v[j] = (j < border ? here : there)[j];
+    for (int j = 0; j < V; ++j) {
+      if (j < until) v.v[j] = here[j];
+      else if (j >= from && j < count) v.v[j] = there[j];
+    }
   }
   bool keep[V];
   if (kDrop) mask_vector<V, Number>(mask, offset, uint64_t(at), keep);
-#pragma unroll
-  for (int j = 0; j < V; ++j)
-    v.v[j] = from_float<T>(!kDrop || keep[j] ? to_float(v.v[j]) * factor : 0.f);
+  v = finish<T, V, kDrop>(v, keep, factor);
   if (at + V <= total) {
     *reinterpret_cast<Vec<T, V>*>(out + at) = v;
   } else {
@@ -165,15 +178,13 @@ cudaError_t run_lookup(const Lookup& a, bool aligned) {
     const int64_t vectors = a.width / V, total = a.n * vectors;
     auto* kernel =
         a.drop ? lookup_kernel<T, Division, V, U, true> : lookup_kernel<T, Division, V, U, false>;
-    kernel<<<grid_of(total, U * kThreads), kThreads, 0, a.stream>>>(
+    return launch_after(kernel, grid_of(total, U * kThreads), kThreads, 0, a.stream,
         Number(total), Division(vectors), table, a.stride, a.index, a.factor, a.mask, out);
-    return cudaGetLastError();
   }
   const int64_t total = a.n * a.width;
   auto go = [&](auto* kernel, int each) {
-    kernel<<<grid_of(total, int64_t(each) * kThreads), kThreads, 0, a.stream>>>(
+    return launch_after(kernel, grid_of(total, int64_t(each) * kThreads), kThreads, 0, a.stream,
         Number(total), Division(a.width), table, a.stride, a.index, a.factor, a.mask, out);
-    return cudaGetLastError();
   };
   if (uint64_t(out) % 16)
     return a.drop ? go(lookup_odd_kernel<T, Division, 1, true, true>, 1)
@@ -220,32 +231,59 @@ const char* problem(int64_t n, int64_t rows, int64_t width, int type, double sca
 
 float factor_of(double scale, double p) { return p < 1.0 ? float(scale / (1.0 - p)) : 0.f; }
 
-template <class T>
-sums::Args<T> sums_of(int64_t n, int64_t rows, int64_t width, const void* grad, int64_t stride,
-                      const uint32_t* order, double scale, double p, uint64_t seed,
-                      uint64_t offset, const int64_t* offset_device, void* workspace) {
-  sums::Args<T> a{};
-  a.n = n;
-  a.rows = rows;
-  a.width = width;
-  a.grad = static_cast<const T*>(grad);
-  a.stride = stride;
-  a.order = reinterpret_cast<const uint2*>(order);
-  a.factor = factor_of(scale, p);
-  a.mask = counter_mask(p, seed, offset, reinterpret_cast<const long long*>(offset_device));
-  a.partial = static_cast<float*>(workspace);
-  return a;
-}
+size_t round_up(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
-const char* sums_problem(int64_t n, int64_t width, const void* grad, int64_t stride,
-                         const uint32_t* order, const void* workspace, size_t bytes,
-                         size_t need) {
-  if (n > 0 && width > 0 && (!grad || !order || !workspace)) return "null array";
-  if (stride < 0) return "bad row stride";
-  if (bytes < need) return "workspace too small";
-  if (uint64_t(workspace) % 16 || uint64_t(order) % 8) return "unaligned workspace or order";
-  return nullptr;
-}
+// What the gradient and Adam entries share: the tokens, checked, and sorted into
+// the front of the workspace unless their order is given.
+struct Tokens {
+  int64_t n, rows, width;
+  Index index;
+  int index_bits;
+  const uint32_t* order;
+  char* workspace;
+  size_t bytes;
+
+  size_t order_bytes() const {
+    return order || n == 0 ? 0
+                           : round_up(size_t(n) * sizeof(uint2)) +
+                                 round_up(tokens::sort_plan(n, rows).bytes());
+  }
+  size_t need(bool consume) const {
+    return order_bytes() +
+           (consume ? sums::consume_bytes(n, rows, width) : n > 0 ? sums::gradient_bytes(n, width) : 0);
+  }
+  const char* problem(const void* grad, int64_t stride, bool consume) const {
+    if (n > 0 && !grad) return "null array";
+    if (stride < 0) return "bad row stride";
+    if (n > 0 && !order) {
+      if (!index.data) return "null array";
+      if (index_bits != 32 && index_bits != 64) return "indices are 32 or 64 bits";
+    }
+    if (need(consume) > 0 && !workspace) return "null array";
+    if (bytes < need(consume)) return "workspace too small";
+    if (uint64_t(workspace) % 256 || uint64_t(order) % 8) return "unaligned workspace or order";
+    return nullptr;
+  }
+  // The arguments of the sums; sorts first where it has to.
+  template <class T>
+  cudaError_t prepare(sums::Args<T>* a, const void* grad, int64_t stride,
+                      const CounterMask& mask, float factor, cudaStream_t stream) const {
+    a->n = n;
+    a->rows = rows;
+    a->width = width;
+    a->grad = static_cast<const T*>(grad);
+    a->stride = stride;
+    a->order = reinterpret_cast<const uint2*>(order);
+    a->factor = factor;
+    a->mask = mask;
+    a->partial = reinterpret_cast<float*>(workspace + order_bytes());
+    if (order || n == 0) return cudaSuccess;
+    uint2* sorted = reinterpret_cast<uint2*>(workspace);
+    a->order = sorted;
+    return tokens::sort_tokens(n, index, sorted, workspace + round_up(size_t(n) * sizeof(uint2)),
+                               stream);
+  }
+};
 
 }  // namespace
 }  // namespace clad3dgs
@@ -297,30 +335,36 @@ extern "C" int clad3dgs_embedding_lookup(int type, int64_t n, int64_t rows, int6
 }
 
 extern "C" size_t clad3dgs_embedding_workspace(int64_t n, int64_t rows, int64_t width,
-                                               int consume) {
+                                               int consume, int ordered) {
   if (n <= 0 || problem(n, rows, width, CLAD3DGS_F32, 1.0, 0.0)) return 0;
-  return consume ? sums::consume_bytes(n, rows, width) : sums::gradient_bytes(n, width);
+  const uint32_t given = 0;
+  const Tokens tokens{n, rows, width, Index{}, 64, ordered ? &given : nullptr, nullptr, 0};
+  return tokens.need(consume != 0);
 }
 
 extern "C" int clad3dgs_embedding_gradient(int type, int64_t n, int64_t rows, int64_t width,
                                            const void* grad, int64_t grad_stride,
-                                           const uint32_t* order, double scale, double p,
-                                           uint64_t seed, uint64_t offset,
+                                           const void* index, int index_bits, int has_padding,
+                                           int64_t padding, const uint32_t* order, double scale,
+                                           double p, uint64_t seed, uint64_t offset,
                                            const int64_t* offset_device, void* out,
                                            void* workspace, size_t workspace_bytes,
                                            cudaStream_t stream) {
   const char* what = "embedding gradient";
   if (const char* why = problem(n, rows, width, type, scale, p)) return refuse(what, why);
   if (rows == 0 || width == 0) return CLAD3DGS_OK;
-  if (const char* why = sums_problem(n, width, grad, grad_stride, order, workspace,
-                                     workspace_bytes, sums::gradient_bytes(n, width)))
-    return refuse(what, why);
+  const Tokens tokens{n, rows, width, Index{index, index_bits == 64, has_padding != 0, padding, rows},
+                      index_bits, order, static_cast<char*>(workspace), workspace_bytes};
+  if (const char* why = tokens.problem(grad, grad_stride, false)) return refuse(what, why);
   if (!out) return refuse(what, "null array");
+  const CounterMask mask =
+      counter_mask(p, seed, offset, reinterpret_cast<const long long*>(offset_device));
   auto go = [&](auto zero) {
     using T = decltype(zero);
-    return sums::gradient(sums_of<T>(n, rows, width, grad, grad_stride, order, scale, p, seed,
-                                     offset, offset_device, workspace),
-                          static_cast<T*>(out), p > 0.0, stream);
+    sums::Args<T> a{};
+    const cudaError_t e =
+        tokens.prepare(&a, grad, grad_stride, mask, factor_of(scale, p), stream);
+    return e == cudaSuccess ? sums::gradient(a, static_cast<T*>(out), p > 0.0, stream) : e;
   };
   return status(what, type == CLAD3DGS_F32   ? go(float())
                       : type == CLAD3DGS_F16 ? go(__half())
@@ -329,26 +373,30 @@ extern "C" int clad3dgs_embedding_gradient(int type, int64_t n, int64_t rows, in
 
 extern "C" int clad3dgs_embedding_consume_torch_adam(
     int type, int64_t n, int64_t rows, int64_t width, const void* grad, int64_t grad_stride,
-    const uint32_t* order, double scale, double p, uint64_t seed, uint64_t offset,
-    const int64_t* offset_device, float* table, float* first, float* second, double rate,
-    TorchAdamConfig config, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+    const void* index, int index_bits, int has_padding, int64_t padding, const uint32_t* order,
+    double scale, double p, uint64_t seed, uint64_t offset, const int64_t* offset_device,
+    float* table, float* first, float* second, double rate, TorchAdamConfig config,
+    void* workspace, size_t workspace_bytes, cudaStream_t stream) {
   const char* what = "embedding consume";
   if (const char* why = problem(n, rows, width, type, scale, p)) return refuse(what, why);
   if (!(std::isfinite(rate) && rate >= 0.0 && config.bias1 > 0.f && config.bias1 <= 1.f &&
         config.bias2_sqrt > 0.f && config.bias2_sqrt <= 1.f))
     return refuse(what, "invalid Adam configuration");
   if (rows == 0 || width == 0) return CLAD3DGS_OK;
-  if (const char* why = sums_problem(n, width, grad, grad_stride, order, workspace,
-                                     workspace_bytes, sums::consume_bytes(n, rows, width)))
-    return refuse(what, why);
+  const Tokens tokens{n, rows, width, Index{index, index_bits == 64, has_padding != 0, padding, rows},
+                      index_bits, order, static_cast<char*>(workspace), workspace_bytes};
+  if (const char* why = tokens.problem(grad, grad_stride, true)) return refuse(what, why);
   if (!table || !first || !second) return refuse(what, "null array");
   const sums::Adam adam{table, first, second, float(rate / double(config.bias1)),
                         1.0 / double(config.bias2_sqrt)};
+  const CounterMask mask =
+      counter_mask(p, seed, offset, reinterpret_cast<const long long*>(offset_device));
   auto go = [&](auto zero) {
     using T = decltype(zero);
-    return sums::consume(sums_of<T>(n, rows, width, grad, grad_stride, order, scale, p, seed,
-                                    offset, offset_device, workspace),
-                         adam, p > 0.0, stream);
+    sums::Args<T> a{};
+    const cudaError_t e =
+        tokens.prepare(&a, grad, grad_stride, mask, factor_of(scale, p), stream);
+    return e == cudaSuccess ? sums::consume(a, adam, p > 0.0, stream) : e;
   };
   return status(what, type == CLAD3DGS_F32   ? go(float())
                       : type == CLAD3DGS_F16 ? go(__half())

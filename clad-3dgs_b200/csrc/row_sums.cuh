@@ -30,6 +30,7 @@
 #include "counter_mask.cuh"
 #include "element_types.cuh"
 #include "gaussian_math.cuh"
+#include "launch.cuh"
 
 namespace clad3dgs {
 namespace sums {
@@ -67,7 +68,7 @@ inline int lanes_of(int64_t vectors, int c, int64_t* padded) {
   return best;
 }
 
-inline Cut cut_of(int64_t n, int64_t width, int vec, int c) {
+inline Cut cut_of(int64_t n, int64_t width, int vec, int c, int64_t rest) {
   const int64_t vectors = (width + vec - 1) / vec;
   Cut cut{};
   int64_t padded;
@@ -75,8 +76,10 @@ inline Cut cut_of(int64_t n, int64_t width, int vec, int c) {
   cut.slices = padded / (cut.lanes * c);
   // Tokens of a group: as many as fill the GPU in whole waves.
   const int groups = kThreads / cut.lanes;
-  const int64_t resident =
-      std::max<int64_t>(1, int64_t(kSms) * blocks_per_sm(c * vec) * groups / cut.slices);
+  // (a few blocks in front for the rows without tokens take places of the first).
+  const int64_t places = int64_t(kSms) * blocks_per_sm(c * vec);
+  const int64_t resident = std::max<int64_t>(
+      1, (places - (rest < places / 2 ? rest : 0)) / cut.slices * groups);
   const int most = std::max(kLeastTokens, kMostTokens / groups);
   const int64_t waves = (n + resident * most - 1) / (resident * most);
   cut.tokens = int(std::max<int64_t>(kLeastTokens, (n + resident * waves - 1) / (resident * waves)));
@@ -231,6 +234,7 @@ enum Head : unsigned char { kNone = 0, kEnded = 1, kOpen = 2 };
 template <class T, int V, int C, int R, bool kDrop, class End>
 __global__ void __launch_bounds__(kThreads, blocks_per_sm(C * V))
     sum_kernel(const __grid_constant__ Args<T> a, const End end) {
+  wait_before();
   if constexpr (End::kRest) {
     if (blockIdx.x < a.rest) {
       write_rest<R, End>(a.n, a.rows, a.width, a.order, end);
@@ -389,46 +393,60 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(C * V))
 
 // Rows that cross borders between blocks: the block that a row begins in adds
 // the heads of the blocks behind it, each group a share of them, the shares in
-// order.
+// order. Bound by latency: what decides is loaded at once.
 template <class T, int V, class End>
 __global__ void __launch_bounds__(kThreads)
     join_kernel(const __grid_constant__ Args<T> a, int lanes, int64_t slices, const End end) {
   __shared__ __align__(16) float shares[kThreads * V];
+  wait_before();
   const int64_t block = blockIdx.x / slices;
   const int64_t first = block * a.cut.block, stop = first + a.cut.block;
   if (stop >= a.n) return;
+  // The row that is open behind this block, and the rows that the next blocks
+  // begin with.
+  int64_t at = stop + int64_t(threadIdx.x) * a.cut.block;
   const uint32_t row = a.order[stop - 1].x;
-  if (row >= a.rows || a.order[stop].x != row) return;
-  if (first > 0 && a.order[first - 1].x == row) return;  // began earlier
+  const uint32_t earlier = first > 0 ? a.order[first - 1].x : kNoRow;
+  uint32_t begins = at < a.n ? a.order[at].x : kNoRow;
+  if (row >= a.rows || earlier == row) return;  // none, or begun earlier
+  int64_t heads = 0;
+  for (;;) {
+    const int more = __syncthreads_count(begins == row);
+    heads += more;
+    if (more < kThreads) break;
+    at += int64_t(kThreads) * a.cut.block;
+    begins = at < a.n ? a.order[at].x : kNoRow;
+  }
+  if (heads == 0) return;
   const int lane = threadIdx.x % lanes, group = threadIdx.x / lanes;
   const int groups = kThreads / lanes;
   const int64_t column = ((blockIdx.x - block * slices) * lanes + lane) * V;
   const bool live = column < a.width;
-  // How many blocks behind begin with this row (they are the next ones).
-  int64_t heads = 0;
-  for (int more = kThreads; more == kThreads; heads += more) {
-    const int64_t at = stop + (heads + threadIdx.x) * a.cut.block;
-    more = __syncthreads_count(at < a.n && a.order[at].x == row);
-  }
-  float sum[V];
+  const float* partial = a.partial + 2 * block * a.width + column;
+  float sum[V], tail[V];
   clear<V>(sum);
-  if (live)
-    for (int64_t h = heads * group / groups; h < heads * (group + 1) / groups; ++h)
-      add<V>(a.partial + 2 * (block + 1 + h) * a.width + column, sum);
+  clear<V>(tail);
+  if (live) {
+    if (group == 0) add<V>(partial + a.width, tail);
+    const int64_t to = heads * (group + 1) / groups;
+#pragma unroll 4
+    for (int64_t h = heads * group / groups; h < to; ++h)
+      add<V>(partial + 2 * (1 + h) * a.width, sum);
+  }
   put<V>(shares + threadIdx.x * V, sum);
   __syncthreads();
   if (group > 0 || !live) return;
-  clear<V>(sum);
-  add<V>(a.partial + (2 * block + 1) * a.width + column, sum);
-  for (int g = 0; g < groups; ++g) add<V>(shares + (g * lanes + lane) * V, sum);
-  scale<V>(sum, a.factor);
-  end.template put<V>(end.place(row, stop - 1, column) * a.width + column, sum);
+  // Groups without a share hold zeros; with few heads most of them do.
+  for (int g = 0; g < groups; ++g) add<V>(shares + (g * lanes + lane) * V, tail);
+  scale<V>(tail, a.factor);
+  end.template put<V>(end.place(row, stop - 1, column) * a.width + column, tail);
 }
 
 // The launch without any token.
 template <int R, class End>
 __global__ void __launch_bounds__(kThreads)
     rest_kernel(int64_t rows, int64_t width, const End end) {
+  wait_before();
   write_rest<R, End>(0, rows, width, nullptr, end);
 }
 
@@ -447,6 +465,7 @@ template <class Division, int W, int U>
 __global__ void __launch_bounds__(kThreads)
     adam_kernel(typename Division::Number total, const Division vectors, int64_t width,
                 const int32_t* __restrict__ slots, const float* __restrict__ sums, const Adam a) {
+  wait_before();
   using Number = typename Division::Number;
   using F = Vec<float, W>;
   const Number first = Number(blockIdx.x) * (U * kThreads) + threadIdx.x;
@@ -502,18 +521,16 @@ inline int vectors_of_lane(int64_t n, int64_t width, int vec, bool floats) {
 
 template <class T, int V, int C, int R, class End>
 cudaError_t run_cut(Args<T> a, const End& end, bool drop, cudaStream_t stream) {
-  a.cut = cut_of(a.n, a.width, V, C);
   a.rest = End::kRest ? rest_blocks(a.rows, a.width, R) : 0;
+  a.cut = cut_of(a.n, a.width, V, C, a.rest);
   const unsigned grid = unsigned(a.rest + a.cut.blocks * a.cut.slices);
   auto* kernel = drop ? sum_kernel<T, V, C, R, true, End> : sum_kernel<T, V, C, R, false, End>;
-  kernel<<<grid, kThreads, 0, stream>>>(a, end);
-  if (a.cut.blocks > 1) {
-    int64_t padded;
-    const int lanes = lanes_of((a.width + V - 1) / V, 1, &padded);
-    join_kernel<T, V, End><<<unsigned(a.cut.blocks * (padded / lanes)), kThreads, 0, stream>>>(
-        a, lanes, padded / lanes, end);
-  }
-  return cudaGetLastError();
+  const cudaError_t e = launch_after(kernel, grid, kThreads, 0, stream, a, end);
+  if (e != cudaSuccess || a.cut.blocks == 1) return e;
+  int64_t padded;
+  const int lanes = lanes_of((a.width + V - 1) / V, 1, &padded);
+  return launch_after(join_kernel<T, V, End>, unsigned(a.cut.blocks * (padded / lanes)), kThreads,
+                      0, stream, a, lanes, padded / lanes, end);
 }
 
 template <class T, int V, int R, class End>
@@ -543,9 +560,8 @@ cudaError_t gradient(const Args<T>& a, T* out, bool drop, cudaStream_t stream) {
   const bool whole = common_bytes(uint64_t(a.width * sizeof(T)) | uint64_t(out)) == 16;
   if (a.n == 0) {
     auto* kernel = whole ? rest_kernel<V, Store<T>> : rest_kernel<1, Store<T>>;
-    kernel<<<unsigned(rest_blocks(a.rows, a.width, whole ? V : 1)), kThreads, 0, stream>>>(
-        a.rows, a.width, end);
-    return cudaGetLastError();
+    return launch_after(kernel, unsigned(rest_blocks(a.rows, a.width, whole ? V : 1)), kThreads, 0,
+                        stream, a.rows, a.width, end);
   }
   if (!whole) return run_sums<T, 1, 1>(a, end, drop, stream);
   return aligned(a) ? run_sums<T, V, V>(a, end, drop, stream)
@@ -575,10 +591,10 @@ cudaError_t run_adam(int64_t rows, int64_t width, const int32_t* slots, const fl
                      const Adam& adam, cudaStream_t stream) {
   constexpr int U = 2;
   const int64_t vectors = width / W, total = rows * vectors;
-  adam_kernel<Division, W, U><<<unsigned((total + U * kThreads - 1) / (U * kThreads)), kThreads, 0,
-                                stream>>>(typename Division::Number(total), Division(vectors),
-                                          width, slots, sums, adam);
-  return cudaGetLastError();
+  return launch_after(adam_kernel<Division, W, U>,
+                      unsigned((total + U * kThreads - 1) / (U * kThreads)), kThreads, 0, stream,
+                      typename Division::Number(total), Division(vectors), width, slots, sums,
+                      adam);
 }
 
 template <class T>

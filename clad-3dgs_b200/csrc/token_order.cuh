@@ -20,6 +20,8 @@
 
 #include <cstdint>
 
+#include "launch.cuh"
+
 namespace clad3dgs {
 namespace tokens {
 
@@ -144,6 +146,7 @@ constexpr int kSmall = kMostBlocks * kSortThreads * 8;
 template <int I>
 __global__ void __launch_bounds__(kSortThreads)
     cluster_sort_kernel(int n, Index index, int passes, int bits, uint2* __restrict__ order) {
+  wait_before();
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = int(cluster.num_blocks()), me = int(cluster.block_rank());
@@ -221,17 +224,19 @@ cudaError_t cluster_sort(int64_t n, const Index& index, uint2* order, cudaStream
   cudaError_t e = cudaFuncSetAttribute(cluster_sort_kernel<I>,
                                        cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared));
   if (e != cudaSuccess) return e;
-  cudaLaunchAttribute attribute{};
-  attribute.id = cudaLaunchAttributeClusterDimension;
-  attribute.val.clusterDim.x = blocks;
-  attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+  cudaLaunchAttribute attributes[2]{};
+  attributes[0].id = cudaLaunchAttributeClusterDimension;
+  attributes[0].val.clusterDim.x = blocks;
+  attributes[0].val.clusterDim.y = attributes[0].val.clusterDim.z = 1;
+  attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // as in launch_after
+  attributes[1].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(blocks);
   config.blockDim = dim3(kSortThreads);
   config.dynamicSmemBytes = shared;
   config.stream = stream;
-  config.attrs = &attribute;
-  config.numAttrs = 1;
+  config.attrs = attributes;
+  config.numAttrs = 2;
   return cudaLaunchKernelEx(&config, cluster_sort_kernel<I>, int(n), index, passes, bits, order);
 }
 
@@ -271,6 +276,7 @@ template <int I>
 __global__ void __launch_bounds__(kSortThreads)
     count_kernel(int64_t n, Index index, const uint2* __restrict__ from, int tiles, int shift,
                  int bits, uint32_t* __restrict__ counts) {
+  wait_before();
   __shared__ uint32_t bins[1 << kSortBits];
   const int digits = 1 << bits;
   for (int d = threadIdx.x; d < digits; d += kSortThreads) bins[d] = 0;
@@ -292,6 +298,7 @@ template <int I>
 __global__ void __launch_bounds__(kSortThreads)
     scatter_kernel(int64_t n, Index index, const uint2* __restrict__ from, int tiles, int shift,
                    int bits, const uint32_t* __restrict__ counts, uint2* __restrict__ to) {
+  wait_before();
   extern __shared__ __align__(16) char shared[];
   const int digits = 1 << bits;
   uint32_t* starts = reinterpret_cast<uint32_t*>(shared);               // [digits]
@@ -374,7 +381,7 @@ cudaError_t large_sort(int64_t n, const Index& index, const SortPlan& p, uint2* 
       reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + p.pair_bytes);
   const size_t shared =
       (size_t(1) << p.bits) * (2 * sizeof(uint32_t) + kSortWarps * sizeof(uint16_t));
-  const cudaError_t e = cudaFuncSetAttribute(
+  cudaError_t e = cudaFuncSetAttribute(
       scatter_kernel<I>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared));
   if (e != cudaSuccess) return e;
   const uint2* from = nullptr;
@@ -382,13 +389,15 @@ cudaError_t large_sort(int64_t n, const Index& index, const SortPlan& p, uint2* 
     // Alternating so that the last pass ends in `order`.
     uint2* to = (p.passes - 1 - pass) % 2 == 0 ? order : spare;
     const int shift = pass * p.bits;
-    count_kernel<I><<<p.blocks, kSortThreads, 0, stream>>>(n, index, from, p.tiles, shift, p.bits,
-                                                           counts);
-    scatter_kernel<I><<<p.blocks, kSortThreads, shared, stream>>>(n, index, from, p.tiles, shift,
-                                                                  p.bits, counts, to);
+    e = launch_after(count_kernel<I>, p.blocks, kSortThreads, 0, stream, n, index, from, p.tiles,
+                     shift, p.bits, counts);
+    if (e != cudaSuccess) return e;
+    e = launch_after(scatter_kernel<I>, p.blocks, kSortThreads, shared, stream, n, index, from,
+                     p.tiles, shift, p.bits, counts, to);
+    if (e != cudaSuccess) return e;
     from = to;
   }
-  return cudaGetLastError();
+  return cudaSuccess;
 }
 
 // Sorts into order[n]; workspace of sort_plan(n, rows).bytes() (none for few

@@ -61,63 +61,74 @@ def row_layout(x):
     return x, x.numel() // width, width, width
 
 
-def on_device(device, call):
-    """call() with `device` current."""
-    if device.index == torch.cuda.current_device():
-        return call()
-    with torch.cuda.device(device):
-        return call()
+def launch(device, what, entry, *arguments):
+    """Calls a C entry on the current stream of `device`, with it current."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        status = entry(*arguments, native.raw_stream(index))
+    else:
+        with torch.cuda.device(device):
+            status = entry(*arguments, native.raw_stream(index))
+    if status:
+        native.check(status, what)
 
 
-def _launch(x, p, seed, offset, rows, out):
-    number, address = check_draw(p, seed, offset, x.device)
+def _run(x, p, seed, number, address, rows, out=None):
+    """The launch, on checked arguments."""
     x, count, width, stride = row_layout(x)
-    if count == 0:
-        return out
-    on_device(x.device, lambda: native.check(native.library().clad3dgs_dropout(
-        TYPES[x.dtype], count, width, x.data_ptr(), stride, out.data_ptr(), width, p, seed,
-        number, address, int(rows), native.stream_handle()), "dropout"))
+    if out is None:
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    if count:
+        launch(x.device, "dropout", native.library().clad3dgs_dropout, TYPES[x.dtype], count,
+               width, x.data_ptr(), stride, out.data_ptr(), width, p, seed, number, address, rows)
     return out
+
+
+def _check(x, p, seed, offset):
+    _require(x.is_cuda, "dropout needs a CUDA tensor")
+    _require(x.dtype in TYPES, "dropout takes float32, float16 or bfloat16")
+    return check_draw(p, seed, offset, x.device)
 
 
 def apply(x, p, seed, offset=0, *, rows=False, out=None):
     """The dropout without autograd. `out`: a contiguous tensor like x to write
     into; x itself (contiguous) for a call in place."""
-    _require(x.is_cuda, "dropout needs a CUDA tensor")
-    _require(x.dtype in TYPES, "dropout takes float32, float16 or bfloat16")
-    if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    else:
+    number, address = _check(x, p, seed, offset)
+    if out is not None:
         _require(out.device == x.device and out.dtype == x.dtype and out.shape == x.shape
                  and out.is_contiguous(), "out must be a contiguous tensor like x")
         same = out.data_ptr() == x.data_ptr() and x.is_contiguous()
-        _require(same or not _overlap(x, out), "out may be x itself, but not overlap it otherwise")
-    return _launch(x, p, seed, offset, rows, out)
+        _require(same or not overlap(x, out), "out may be x itself, but not overlap it otherwise")
+    return _run(x.detach(), p, seed, number, address, bool(rows), out)
 
 
-def _overlap(x, out):
-    if x.numel() == 0:
+def overlap(x, y):
+    """Whether the memory between the first and the last element of x meets y's."""
+    if x.numel() == 0 or y.numel() == 0:
         return False
-    first = x.data_ptr()
-    last = first + x.element_size() * (1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride())))
-    return first < out.data_ptr() + out.numel() * out.element_size() and out.data_ptr() < last
+    spans = []
+    for t in (x, y):
+        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+        spans.append((t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()))
+    return spans[0][0] < spans[1][1] and spans[1][0] < spans[0][1]
 
 
 class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, p, seed, offset, rows):
-        ctx.numbers = p, seed, rows
-        if isinstance(offset, torch.Tensor):
+        number, address = _check(x, p, seed, offset)
+        ctx.numbers = p, seed, offset if address is None else None, rows
+        if address is not None:
             ctx.save_for_backward(offset)
-            ctx.offset = None
-        else:
-            ctx.offset = offset
-        return apply(x, p, seed, offset, rows=rows)
+        return _run(x, p, seed, number, address, rows)
 
     @staticmethod
     def backward(ctx, grad):
-        p, seed, rows = ctx.numbers
-        offset = ctx.saved_tensors[0] if ctx.offset is None else ctx.offset
+        p, seed, offset, rows = ctx.numbers
+        if offset is None:
+            offset = ctx.saved_tensors[0]
+        elif not torch.is_grad_enabled():
+            return _run(grad, p, seed, offset, None, rows), None, None, None, None
         return dropout(grad, p, seed, offset, rows=rows), None, None, None, None
 
 
@@ -125,5 +136,6 @@ def dropout(x, p, seed, offset=0, *, rows=False):
     """x with a share p of its elements (rows=True: of its rows) set to zero and
     the others scaled by 1 / (1 - p); differentiable any number of times."""
     if x.requires_grad and torch.is_grad_enabled():
-        return _Dropout.apply(x, p, seed, offset, rows)
-    return apply(x, p, seed, offset, rows=rows)
+        return _Dropout.apply(x, p, seed, offset, bool(rows))
+    number, address = _check(x, p, seed, offset)
+    return _run(x, p, seed, number, address, bool(rows))

@@ -37,7 +37,7 @@ import torch
 
 import _native as native
 from consume import check_disjoint
-from dropout import TYPES, check_draw, on_device
+from dropout import TYPES, check_draw, launch, overlap
 
 MOST = 2 ** 31 - 1
 _BITS = {torch.int32: 32, torch.int64: 64}
@@ -54,15 +54,17 @@ class TokenOrder(NamedTuple):
     rows: int
 
 
-def _check_index(index, device):
+def _index(index, device):
+    """The checked index: (tensor, bits)."""
     _require(index.is_cuda and (device is None or index.device == device),
              "index must be on the tensors' CUDA device")
-    _require(index.dtype in _BITS, "index must be int32 or int64")
+    bits = _BITS.get(index.dtype)
+    _require(bits is not None, "index must be int32 or int64")
     _require(index.numel() <= MOST, "at most 2^31 - 1 tokens")
-    return index if index.is_contiguous() else index.contiguous()
+    return index if index.is_contiguous() else index.contiguous(), bits
 
 
-def _check_padding(padding_index):
+def _padding(padding_index):
     if padding_index is None:
         return 0, 0
     _require(isinstance(padding_index, int) and -2 ** 63 <= padding_index < 2 ** 63,
@@ -74,64 +76,82 @@ def _check_scale(scale):
     _require(isinstance(scale, (int, float)) and math.isfinite(scale), "scale must be finite")
 
 
+def _check_rows(rows):
+    _require(isinstance(rows, int) and 0 <= rows <= MOST, "rows must be in [0, 2^31)")
+
+
 def _matrix(t, name):
-    """t as a matrix with unit column stride: (tensor, rows, width, row stride)."""
-    _require(t.is_cuda and t.dtype in TYPES, f"{name} must be CUDA float32, float16 or bfloat16")
+    """t as a matrix with unit column stride: (tensor, type, rows, width, row
+    stride)."""
+    kind = TYPES.get(t.dtype)
+    _require(t.is_cuda and kind is not None, f"{name} must be CUDA float32, float16 or bfloat16")
     _require(t.dim() == 2, f"{name} must be a matrix")
-    if t.stride(1) != 1 and t.shape[1] > 1:
+    rows, width = t.shape
+    if t.is_contiguous():
+        return t, kind, rows, width, width
+    if t.stride(1) != 1 and width > 1:
         t = t.contiguous()
-    return t, t.shape[0], t.shape[1], t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    return t, kind, rows, width, t.stride(0)
 
 
-def _bytes(count, device):
-    return torch.empty(max(count, 1), dtype=torch.uint8, device=device)
+def _gradient_matrix(grad):
+    """Output gradients [*, width] as a matrix, one row per token."""
+    _require(grad.dim() >= 1, "grad must have one row per token")
+    if grad.dim() != 2:
+        rows = math.prod(grad.shape[:-1])
+        grad = grad.reshape(rows, grad.shape[-1])
+    return _matrix(grad, "grad")
 
 
 def token_order(index, rows, *, padding_index=None):
     """The tokens of `index` (row-major) sorted by row, for `lookup_gradient` and
     `consume_torch_adam` on a table of `rows` rows."""
-    index = _check_index(index, None)
-    _require(isinstance(rows, int) and 0 <= rows <= MOST, "rows must be in [0, 2^31)")
-    padded, padding = _check_padding(padding_index)
-    n, device = index.numel(), index.device
-    pairs = torch.empty((n, 2), dtype=torch.int32, device=device)
-    if n == 0:
-        return TokenOrder(pairs, rows)
-    lib = native.library()
-    workspace = _bytes(lib.clad3dgs_token_order_workspace(n, rows), device)
-    on_device(device, lambda: native.check(lib.clad3dgs_token_order(
-        n, rows, index.data_ptr(), _BITS[index.dtype], padded, padding, pairs.data_ptr(),
-        workspace.data_ptr(), workspace.numel(), native.stream_handle()), "token order"))
+    index, bits = _index(index, None)
+    _check_rows(rows)
+    padded, padding = _padding(padding_index)
+    n = index.numel()
+    pairs = index.new_empty((n, 2), dtype=torch.int32)
+    if n:
+        lib = native.library()
+        need = lib.clad3dgs_token_order_workspace(n, rows)
+        workspace = index.new_empty(need, dtype=torch.uint8) if need else None
+        launch(index.device, "token order", lib.clad3dgs_token_order, n, rows, index.data_ptr(),
+               bits, padded, padding, pairs.data_ptr(), native.ptr(workspace), need)
     return TokenOrder(pairs, rows)
 
 
-def _order_of(index, rows, padding_index, order, tokens, device):
-    """The checked order of `tokens` tokens, sorted here if it is not given."""
+def _tokens(index, rows, padding_index, order, count, device):
+    """The tokens as the C entries take them (index, bits, has padding, padding,
+    order), and the tensor that has to live until the launch."""
     if order is None:
-        _require(index.numel() == tokens, "grad must have one row per token")
-        _require(index.device == device, "index must be on the tensors' CUDA device")
-        return token_order(index, rows, padding_index=padding_index)
+        index, bits = _index(index, device)
+        _require(index.numel() == count, "grad must have one row per token")
+        return (native.ptr(index), bits, *_padding(padding_index), None), index
     _require(isinstance(order, TokenOrder) and order.rows == rows
-             and order.pairs.shape[0] == tokens and order.pairs.device == device,
+             and order.pairs.shape[0] == count and order.pairs.device == device,
              "the token order belongs to another table, device or number of tokens")
-    return order
+    return (None, 0, 0, 0, native.ptr(order.pairs)), order.pairs
+
+
+def _workspace(count, rows, width, consume, ordered, device):
+    need = native.library().clad3dgs_embedding_workspace(count, rows, width, consume, ordered)
+    return torch.empty(need, dtype=torch.uint8, device=device), need
 
 
 def _lookup(table, index, scale, padding_index, p, seed, offset):
-    table, rows, width, stride = _matrix(table, "table")
+    table, kind, rows, width, stride = _matrix(table, "table")
+    device = table.device
     shape = (*index.shape, width)
-    index = _check_index(index, table.device)
-    _require(rows <= MOST, "at most 2^31 - 1 rows")
+    index, bits = _index(index, device)
+    _check_rows(rows)
     _check_scale(scale)
-    padded, padding = _check_padding(padding_index)
-    number, address = check_draw(p, seed, offset, table.device)
-    out = torch.empty(shape, dtype=table.dtype, device=table.device)
+    padded, padding = _padding(padding_index)
+    number, address = check_draw(p, seed, offset, device)
+    out = table.new_empty(shape)
     if out.numel():
-        on_device(table.device, lambda: native.check(
-            native.library().clad3dgs_embedding_lookup(
-                TYPES[table.dtype], index.numel(), rows, width, native.ptr(table), stride,
-                index.data_ptr(), _BITS[index.dtype], padded, padding, scale, p, seed, number,
-                address, out.data_ptr(), native.stream_handle()), "embedding lookup"))
+        launch(device, "embedding lookup", native.library().clad3dgs_embedding_lookup, kind,
+               index.numel(), rows, width, table.data_ptr(), stride, index.data_ptr(), bits,
+               padded, padding, scale, p, seed, number, address, out.data_ptr())
     return out
 
 
@@ -140,24 +160,18 @@ def lookup_gradient(grad, index, rows, *, scale=1.0, padding_index=None, p=0.0, 
     """The table's gradient [rows, width] (grad's type) of a `lookup` with these
     arguments whose output has the gradient `grad` [*index.shape, width]. With
     `order` (from `token_order`), index and padding_index are not read."""
-    _require(grad.dim() >= 1, "grad must have one row per token")
-    grad, tokens, width, stride = _matrix(grad if grad.dim() == 2
-                                          else grad.reshape(-1, grad.shape[-1])
-                                          if grad.numel() else
-                                          grad.new_empty(0, grad.shape[-1]), "grad")
-    _check_scale(scale)
+    grad, kind, count, width, stride = _gradient_matrix(grad)
     device = grad.device
+    _check_rows(rows)
+    _check_scale(scale)
     number, address = check_draw(p, seed, offset, device)
-    order = _order_of(index, rows, padding_index, order, tokens, device)
-    out = torch.empty((rows, width), dtype=grad.dtype, device=device)
-    if out.numel() == 0:
-        return out
-    lib = native.library()
-    workspace = _bytes(lib.clad3dgs_embedding_workspace(tokens, rows, width, 0), device)
-    on_device(device, lambda: native.check(lib.clad3dgs_embedding_gradient(
-        TYPES[grad.dtype], tokens, rows, width, native.ptr(grad), stride,
-        native.ptr(order.pairs), scale, p, seed, number, address, out.data_ptr(),
-        workspace.data_ptr(), workspace.numel(), native.stream_handle()), "embedding gradient"))
+    tokens, alive = _tokens(index, rows, padding_index, order, count, device)
+    out = grad.new_empty((rows, width))
+    if out.numel():
+        workspace, need = _workspace(count, rows, width, 0, order is not None, device)
+        launch(device, "embedding gradient", native.library().clad3dgs_embedding_gradient, kind,
+               count, rows, width, native.ptr(grad), stride, *tokens, scale, p, seed, number,
+               address, out.data_ptr(), native.ptr(workspace), need)
     return out
 
 
@@ -168,54 +182,49 @@ def consume_torch_adam(table, first, second, grad, index, *, rate, bias1, bias2_
     gradient that `lookup_gradient` would give in 32 bits. Rows without tokens
     are updated with a zero gradient. Like the other consume entries it does
     not touch step counters or autograd versions."""
-    _require(grad.dim() >= 1, "grad must have one row per token")
-    grad, tokens, width, stride = _matrix(grad if grad.dim() == 2
-                                          else grad.reshape(-1, grad.shape[-1])
-                                          if grad.numel() else
-                                          grad.new_empty(0, grad.shape[-1]), "grad")
+    grad, kind, count, width, stride = _gradient_matrix(grad)
     device = grad.device
-    for name, t in (("table", table), ("first", first), ("second", second)):
-        _require(t.is_cuda and t.device == device and t.dtype == torch.float32
-                 and t.dim() == 2 and t.shape == table.shape and t.is_contiguous(),
-                 f"{name} must be contiguous CUDA float32 [rows, width] on grad's device")
+    _require(table.dim() == 2, "table must be a matrix")
     rows = table.shape[0]
-    _require(table.shape[1] == width, "grad and table must have the same width")
+    for name, t in (("table", table), ("first", first), ("second", second)):
+        _require(t.dtype == torch.float32 and t.device == device and t.shape == (rows, width)
+                 and t.is_contiguous(),
+                 f"{name} must be contiguous CUDA float32 [rows, width] on grad's device")
+    _check_rows(rows)
     _check_scale(scale)
     _require(math.isfinite(rate) and rate >= 0 and 0 < bias1 <= 1 and 0 < bias2_sqrt <= 1,
              "invalid Adam configuration")
     number, address = check_draw(p, seed, offset, device)
-    check_disjoint([table, first, second], [grad] if order is None else [grad, order.pairs],
-                   "table, moments and gradient must be disjoint")
-    order = _order_of(index, rows, padding_index, order, tokens, device)
-    if table.numel() == 0:
-        return
-    lib = native.library()
-    workspace = _bytes(lib.clad3dgs_embedding_workspace(tokens, rows, width, 1), device)
-    on_device(device, lambda: native.check(lib.clad3dgs_embedding_consume_torch_adam(
-        TYPES[grad.dtype], tokens, rows, width, native.ptr(grad), stride,
-        native.ptr(order.pairs), scale, p, seed, number, address, table.data_ptr(),
-        first.data_ptr(), second.data_ptr(), rate, native.TorchAdamConfig(bias1, bias2_sqrt),
-        workspace.data_ptr(), workspace.numel(), native.stream_handle()), "embedding consume"))
+    tokens, alive = _tokens(index, rows, padding_index, order, count, device)
+    check_disjoint([table, first, second], [alive],
+                   "table, moments and indices must be disjoint")
+    _require(not any(overlap(grad, t) for t in (table, first, second)),
+             "table, moments and gradient must be disjoint")
+    if table.numel():
+        workspace, need = _workspace(count, rows, width, 1, order is not None, device)
+        launch(device, "embedding consume", native.library().clad3dgs_embedding_consume_torch_adam,
+               kind, count, rows, width, native.ptr(grad), stride, *tokens, scale, p, seed, number,
+               address, table.data_ptr(), first.data_ptr(), second.data_ptr(), rate,
+               native.TorchAdamConfig(bias1, bias2_sqrt), native.ptr(workspace), need)
 
 
 class _Lookup(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, index, scale, padding_index, p, seed, offset, order):
-        ctx.numbers = table.shape[0], scale, padding_index, p, seed, order
         tensor = isinstance(offset, torch.Tensor)
-        ctx.offset = None if tensor else offset
-        ctx.save_for_backward(index, *([offset] if tensor else []))
+        ctx.numbers = (table.shape[0], scale, padding_index, p, seed, None if tensor else offset,
+                       order)
+        ctx.save_for_backward(index, *((offset,) if tensor else ()))
         return _lookup(table, index, scale, padding_index, p, seed, offset)
 
     @staticmethod
     def backward(ctx, grad):
         if torch.is_grad_enabled():
             raise RuntimeError("embedding lookup supports first-order backward only")
-        rows, scale, padding_index, p, seed, order = ctx.numbers
+        rows, scale, padding_index, p, seed, offset, order = ctx.numbers
         index, *tensor = ctx.saved_tensors
-        offset = tensor[0] if tensor else ctx.offset
-        return (lookup_gradient(grad, index, rows, scale=scale, padding_index=padding_index,
-                                p=p, seed=seed, offset=offset, order=order),
+        return (lookup_gradient(grad, index, rows, scale=scale, padding_index=padding_index, p=p,
+                                seed=seed, offset=tensor[0] if tensor else offset, order=order),
                 None, None, None, None, None, None, None)
 
 
@@ -225,6 +234,6 @@ def lookup(table, index, *, scale=1.0, padding_index=None, p=0.0, seed=0, offset
     of the same index, rows and padding) spares the backward pass its sort."""
     if table.requires_grad and torch.is_grad_enabled():
         if order is not None:
-            _order_of(index, table.shape[0], padding_index, order, index.numel(), table.device)
+            _tokens(None, table.shape[0], None, order, index.numel(), table.device)
         return _Lookup.apply(table, index, scale, padding_index, p, seed, offset, order)
     return _lookup(table, index, scale, padding_index, p, seed, offset)

@@ -529,27 +529,32 @@ int clad3dgs_embedding_lookup(int type, int64_t n, int64_t rows, int64_t width,
 /* The lookup's adjoint: out[k] = scale * sum over tokens i of row k of
  * grad[i] (through the dropout of the same p, seed and offset), [rows][width]
  * of grad's type, every row written (zeros where no token names it). grad
- * [n][width] with a row stride in elements; order from clad3dgs_token_order of
- * the same n and rows. Sums are 32-bit floats in an order that depends on
- * the sizes alone. workspace: clad3dgs_embedding_workspace bytes (consume = 0
- * here, 1 for the Adam entry below), 16-byte aligned. */
-size_t clad3dgs_embedding_workspace(int64_t n, int64_t rows, int64_t width, int consume);
+ * [n][width] with a row stride in elements. The tokens are given by order, from
+ * clad3dgs_token_order of the same n and rows, or with order null by index,
+ * index_bits and padding (as there), which the call then sorts for itself. Sums
+ * are 32-bit floats in an order that depends on the sizes alone. workspace:
+ * clad3dgs_embedding_workspace bytes (consume = 0 here, 1 for the Adam entry
+ * below; ordered = whether order is given), 256-byte aligned. */
+size_t clad3dgs_embedding_workspace(int64_t n, int64_t rows, int64_t width, int consume,
+                                    int ordered);
 int clad3dgs_embedding_gradient(int type, int64_t n, int64_t rows, int64_t width,
-                                const void* grad, int64_t grad_stride, const uint32_t* order,
-                                double scale, double p, uint64_t seed, uint64_t offset,
-                                const int64_t* offset_device, void* out, void* workspace,
-                                size_t workspace_bytes, cudaStream_t stream);
+                                const void* grad, int64_t grad_stride, const void* index,
+                                int index_bits, int has_padding, int64_t padding,
+                                const uint32_t* order, double scale, double p, uint64_t seed,
+                                uint64_t offset, const int64_t* offset_device, void* out,
+                                void* workspace, size_t workspace_bytes, cudaStream_t stream);
 
 /* The adjoint handed to torch-fused Adam (rate, bias corrections as elsewhere
  * in this header): table and both moments [rows][width], float, updated in
  * place; of the table's gradient only the rows that tokens name exist, in the
- * workspace. Dense: the other rows are updated with a gradient of zero. The arrays must be disjoint
- * from each other and from grad. */
+ * workspace. Dense: the other rows are updated with a gradient of zero. The
+ * arrays must be disjoint from each other and from grad. */
 int clad3dgs_embedding_consume_torch_adam(
     int type, int64_t n, int64_t rows, int64_t width, const void* grad, int64_t grad_stride,
-    const uint32_t* order, double scale, double p, uint64_t seed, uint64_t offset,
-    const int64_t* offset_device, float* table, float* first, float* second, double rate,
-    TorchAdamConfig config, void* workspace, size_t workspace_bytes, cudaStream_t stream);
+    const void* index, int index_bits, int has_padding, int64_t padding, const uint32_t* order,
+    double scale, double p, uint64_t seed, uint64_t offset, const int64_t* offset_device,
+    float* table, float* first, float* second, double rate, TorchAdamConfig config,
+    void* workspace, size_t workspace_bytes, cudaStream_t stream);
 
 #ifdef __cplusplus
 }

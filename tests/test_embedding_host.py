@@ -24,9 +24,9 @@ ORDER = dict(n=200_000, rows=4, index=256, index_bits=64, has_padding=0, padding
 LOOKUP = dict(type=0, n=10, rows=4, width=8, table=256, table_stride=8, index=512, index_bits=64,
               has_padding=0, padding=0, scale=1.0, p=0.0, seed=0, offset=0, offset_device=None,
               out=1024, stream=0)
-GRADIENT = dict(type=0, n=10, rows=4, width=8, grad=256, grad_stride=8, order=512, scale=1.0, p=0.0,
-                seed=0, offset=0, offset_device=None, out=1024, workspace=2048,
-                workspace_bytes=1 << 20, stream=0)
+GRADIENT = dict(type=0, n=10, rows=4, width=8, grad=256, grad_stride=8, index=None, index_bits=0,
+                has_padding=0, padding=0, order=512, scale=1.0, p=0.0, seed=0, offset=0,
+                offset_device=None, out=1024, workspace=2048, workspace_bytes=1 << 20, stream=0)
 NAN, INF = float("nan"), float("inf")
 
 
@@ -44,7 +44,9 @@ SHARED = [dict(n=-1), dict(rows=-1), dict(n=2 ** 31), dict(rows=2 ** 31)]
 SIZED = SHARED + [dict(width=-1), dict(type=3), dict(type=-1), dict(scale=INF), dict(scale=NAN),
                   dict(p=-0.5), dict(p=1.5), dict(p=NAN), dict(n=2 ** 30, width=2 ** 40)]
 SUMS = SIZED + [dict(grad=None), dict(order=None), dict(workspace=None), dict(workspace_bytes=8),
-                dict(grad_stride=-1), dict(workspace=2056), dict(order=516)]
+                dict(grad_stride=-1), dict(workspace=2064), dict(order=516),
+                dict(order=None, index=256, index_bits=16),
+                dict(order=None, index=256, index_bits=64, workspace_bytes=300)]
 
 
 @pytest.mark.parametrize("entry,change", (
@@ -99,11 +101,13 @@ def test_workspaces():
     lib = native.library()
     assert lib.clad3dgs_token_order_workspace(0, 5) == 0
     assert lib.clad3dgs_token_order_workspace(2 ** 31, 5) == 0
-    assert lib.clad3dgs_embedding_workspace(0, 5, 5, 0) == 0
-    assert lib.clad3dgs_embedding_workspace(5, -1, 5, 0) == 0
-    assert lib.clad3dgs_embedding_workspace(2 ** 31, 5, 5, 1) == 0
+    assert lib.clad3dgs_embedding_workspace(0, 5, 5, 0, 1) == 0
+    assert lib.clad3dgs_embedding_workspace(5, -1, 5, 0, 1) == 0
+    assert lib.clad3dgs_embedding_workspace(2 ** 31, 5, 5, 1, 1) == 0
     sizes = [lib.clad3dgs_token_order_workspace(n, 4096) for n in (1, 10_000, 70_000, 1_000_000)]
     assert sizes == sorted(sizes) and sizes[2] > 0  # few tokens need none
-    few, many = (lib.clad3dgs_embedding_workspace(n, 4096, 48, 0) for n in (10, 1_000_000))
+    assert (lib.clad3dgs_embedding_workspace(70_000, 5, 5, 0, 0)
+            >= lib.clad3dgs_embedding_workspace(70_000, 5, 5, 0, 1) + 8 * 70_000)
+    few, many = (lib.clad3dgs_embedding_workspace(n, 4096, 48, 0, 1) for n in (10, 1_000_000))
     assert 0 < few < many
-    assert lib.clad3dgs_embedding_workspace(10, 4096, 48, 1) >= few + 4 * 4096 + 10 * 48 * 4
+    assert lib.clad3dgs_embedding_workspace(10, 4096, 48, 1, 1) >= few + 4 * 4096 + 10 * 48 * 4
