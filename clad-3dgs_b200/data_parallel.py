@@ -63,6 +63,7 @@ import torch
 import torch.distributed as dist
 
 import _native as native
+import dropout
 
 GROUPS = (("xyz", 3), ("sh", 48), ("scaling", 3), ("rotation", 4), ("opacity", 1))
 WIDTH = dict(GROUPS)
@@ -567,12 +568,22 @@ class _Scratch:
 class DataParallelTrainer:
     """One training step per call: this rank renders its camera, takes the L1
     loss against its target, back-propagates into its gradient arrays, and the
-    ranks exchange and update (ShardedAdam.step)."""
+    ranks exchange and update (ShardedAdam.step).
+
+    `opacity_dropout` p > 0 drops each Gaussian from a view with probability p
+    (a regularisation for few views): the renderer gets the activated opacity
+    through `dropout.dropout` under `dropout_seed`, with a fresh offset for every
+    step and rank, and the opacity's gradient goes back through the same draw.
+    The update itself uses the undropped opacity, as always."""
 
     def __init__(self, values, rates=None, *, degree=3, bg=(0.0, 0.0, 0.0), group=None,
                  exchange=None, device=None, pixel_accumulation=2, sh_exchange=None,
-                 gate=None):
+                 gate=None, opacity_dropout=0.0, dropout_seed=0):
         n = int(values["xyz"].shape[0])
+        if not 0.0 <= opacity_dropout < 1.0:
+            raise ValueError("opacity_dropout must lie in [0, 1)")
+        if not (isinstance(dropout_seed, int) and 0 <= dropout_seed < 2 ** 64):
+            raise ValueError("dropout_seed must be an integer in [0, 2^64)")
         self.adam = ShardedAdam(n, rates, group=group, exchange=exchange, device=device,
                                 sh_exchange=sh_exchange, degree=degree, gate=gate)
         self.adam.load(values)
@@ -590,6 +601,8 @@ class DataParallelTrainer:
         self.radii = torch.zeros(n, dtype=torch.int32, device=dev)
         self.loss = z(1)
         self.buffers = _Scratch(dev)
+        self.opacity_dropout, self.dropout_seed = float(opacity_dropout), dropout_seed
+        self._dropped = z(self.adam.padded, 1) if opacity_dropout > 0 else None
         self.image = self.dimage = None
         self._declared = None  # colour form: the camera the colours were made for
 
@@ -639,6 +652,11 @@ class DataParallelTrainer:
             self._declared = next_camera
         return loss, rendered
 
+    def _drop(self, x, out):
+        """This step's opacity dropout on this rank (it is its own adjoint)."""
+        offset = self.adam.t * self.adam.world + self.adam.rank
+        dropout.apply(x, self.opacity_dropout, self.dropout_seed, offset, out=out)
+
     def backward(self, camera: Camera, target):
         """Everything of a step before the exchange: this rank's gradients."""
         lib, a = native.library(), self.adam
@@ -656,6 +674,10 @@ class DataParallelTrainer:
         self._accumulated.zero_()
         self.loss.zero_()
         act = a.activate()
+        opacity = act["opacity"]
+        if self._dropped is not None:
+            self._drop(opacity, self._dropped)
+            opacity = self._dropped
         p = a.params
         # Colour form: the owners' colours for this view stand for the SH.
         colours = a.colours.data_ptr() if a.sh_exchange == "colours" else None
@@ -663,7 +685,7 @@ class DataParallelTrainer:
         rendered = ctypes.c_int(0)
         native.check(lib.clad3dgs_raster_forward(
             n, self.degree, self.bg.data_ptr(), p["xyz"].data_ptr(), colours,
-            act["opacity"].data_ptr(), act["scaling"].data_ptr(), 1.0,
+            opacity.data_ptr(), act["scaling"].data_ptr(), 1.0,
             act["rotation"].data_ptr(), None, camera.view.data_ptr(), camera.proj.data_ptr(),
             camera.tan_x, camera.tan_y, H, W, sh, None, None,
             camera.campos.data_ptr(), 0, ctypes.cast(self.buffers.callback, ctypes.c_void_p),
@@ -679,7 +701,7 @@ class DataParallelTrainer:
         binning = self.buffers.tensors.get(2)
         native.check(lib.clad3dgs_raster_backward(
             n, self.degree, self.bg.data_ptr(), p["xyz"].data_ptr(), self.radii.data_ptr(),
-            colours, act["opacity"].data_ptr(), act["scaling"].data_ptr(), 1.0,
+            colours, opacity.data_ptr(), act["scaling"].data_ptr(), 1.0,
             act["rotation"].data_ptr(), None, camera.view.data_ptr(), camera.proj.data_ptr(),
             camera.tan_x, camera.tan_y, H, W, self.dimage.data_ptr(),
             None, sh, None, None,
@@ -691,6 +713,8 @@ class DataParallelTrainer:
             None, self.mode, 2 if seeded else 0, None, None, None, None, None, None,
             native.TorchAdamConfig(1.0, 1.0), None, None, 0.0, native.TorchAdamConfig(1.0, 1.0),
             stream), "rasterize (backward)")
+        if self._dropped is not None:
+            self._drop(g["opacity"], g["opacity"])
         if seeded:
             # This view's colour seeds and camera for the SH backward in the update.
             native.check(lib.clad3dgs_raster_sh_seeds(
