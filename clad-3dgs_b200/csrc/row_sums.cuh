@@ -37,7 +37,7 @@ namespace sums {
 
 constexpr int kThreads = 256;
 constexpr int kSms = 148;
-constexpr int kMostTokens = 2560;  // of a block: their order entries lie in shared memory
+constexpr int kMostTokens = 3584;  // of a block: their order entries lie in shared memory
 constexpr int kLeastTokens = 8;    // of a group: keeps the joins few
 constexpr uint32_t kNoRow = ~0u;
 
@@ -399,8 +399,8 @@ __global__ void __launch_bounds__(kThreads)
     join_kernel(const __grid_constant__ Args<T> a, int lanes, int64_t slices, const End end) {
   __shared__ __align__(16) float shares[kThreads * V];
   wait_before();
-  const int64_t block = blockIdx.x / slices;
-  const int64_t first = block * a.cut.block, stop = first + a.cut.block;
+  const unsigned block = blockIdx.x / unsigned(slices);
+  const int64_t first = int64_t(block) * a.cut.block, stop = first + a.cut.block;
   if (stop >= a.n) return;
   // The row that is open behind this block, and the rows that the next blocks
   // begin with.
@@ -409,7 +409,7 @@ __global__ void __launch_bounds__(kThreads)
   const uint32_t earlier = first > 0 ? a.order[first - 1].x : kNoRow;
   uint32_t begins = at < a.n ? a.order[at].x : kNoRow;
   if (row >= a.rows || earlier == row) return;  // none, or begun earlier
-  int64_t heads = 0;
+  int heads = 0;
   for (;;) {
     const int more = __syncthreads_count(begins == row);
     heads += more;
@@ -420,24 +420,25 @@ __global__ void __launch_bounds__(kThreads)
   if (heads == 0) return;
   const int lane = threadIdx.x % lanes, group = threadIdx.x / lanes;
   const int groups = kThreads / lanes;
-  const int64_t column = ((blockIdx.x - block * slices) * lanes + lane) * V;
+  const int64_t column = (int64_t(blockIdx.x - block * unsigned(slices)) * lanes + lane) * V;
   const bool live = column < a.width;
-  const float* partial = a.partial + 2 * block * a.width + column;
+  const float* partial = a.partial + 2 * int64_t(block) * a.width + column;
   float sum[V], tail[V];
   clear<V>(sum);
   clear<V>(tail);
-  if (live) {
+  const int sharing = heads < groups ? heads : groups;
+  if (live && group < sharing) {
     if (group == 0) add<V>(partial + a.width, tail);
-    const int64_t to = heads * (group + 1) / groups;
+    const int each = heads / sharing, more = heads % sharing;  // the first ones take one more
+    const int from = group * each + (group < more ? group : more);
+    const int to = from + each + (group < more ? 1 : 0);
 #pragma unroll 4
-    for (int64_t h = heads * group / groups; h < to; ++h)
-      add<V>(partial + 2 * (1 + h) * a.width, sum);
+    for (int h = from; h < to; ++h) add<V>(partial + 2 * int64_t(1 + h) * a.width, sum);
   }
   put<V>(shares + threadIdx.x * V, sum);
   __syncthreads();
   if (group > 0 || !live) return;
-  // Groups without a share hold zeros; with few heads most of them do.
-  for (int g = 0; g < groups; ++g) add<V>(shares + (g * lanes + lane) * V, tail);
+  for (int g = 0; g < sharing; ++g) add<V>(shares + (g * lanes + lane) * V, tail);
   scale<V>(tail, a.factor);
   end.template put<V>(end.place(row, stop - 1, column) * a.width + column, tail);
 }

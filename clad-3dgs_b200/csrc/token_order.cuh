@@ -87,10 +87,10 @@ __device__ __forceinline__ void rank_tile(const uint2 (&pair)[I], int count, int
   uint32_t same[I];
 #pragma unroll
   for (int j = 0; j < I; ++j) same[j] = __ballot_sync(~0u, base + 32 * j < count);
-  for (int b = shift; b < shift + bits; ++b) {
+  for (uint32_t bit = 1u << shift, end = bit << bits; bit != end; bit <<= 1) {
 #pragma unroll
     for (int j = 0; j < I; ++j) {
-      const bool set = b < 32 && (pair[j].x >> b & 1);
+      const bool set = (pair[j].x & bit) != 0;
       const uint32_t lanes = __ballot_sync(~0u, set);
       same[j] &= set ? lanes : ~lanes;
     }
