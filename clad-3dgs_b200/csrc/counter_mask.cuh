@@ -72,6 +72,19 @@ __device__ __forceinline__ uint32_t word_of(const uint4& w, unsigned j) {
   return j == 0 ? w.x : j == 1 ? w.y : j == 2 ? w.z : w.w;
 }
 
+// The decisions for four elements that begin at any element e.
+__device__ __forceinline__ void mask_four(const CounterMask& m, unsigned long long offset,
+                                          uint64_t e, bool (&keep)[4]) {
+  const unsigned shift = unsigned(e) % 4;
+  const uint4 a = mask_words(m, offset, e / 4);
+  uint4 b = make_uint4(0, 0, 0, 0);
+  if (shift) b = mask_words(m, offset, e / 4 + 1);
+  const uint32_t w[7] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z};
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    keep[j] = m.keeps(shift == 0 ? w[j] : shift == 1 ? w[j + 1] : shift == 2 ? w[j + 2] : w[j + 3]);
+}
+
 // The decisions for V elements that begin at element e, e a multiple of V (a
 // multiple of four, or V = 1). Number: uint32_t where every e / 4 fits one.
 template <int V, class Number = uint64_t>

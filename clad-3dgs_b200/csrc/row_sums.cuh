@@ -41,8 +41,11 @@ constexpr int kMostTokens = 3584;  // of a block: their order entries lie in sha
 constexpr int kLeastTokens = 8;    // of a group: keeps the joins few
 constexpr uint32_t kNoRow = ~0u;
 
-// Rows a thread asks for at once, and the blocks that an SM's registers hold.
-constexpr int rows_at_once(int c) { return c == 1 ? 4 : 2; }
+// Rows a thread asks for at once (of each it takes `bytes`), and the blocks that
+// an SM's registers hold.
+constexpr int rows_at_once(int bytes, bool loose) {
+  return loose ? 2 : bytes <= 8 ? 8 : bytes <= 16 ? 4 : 2;
+}
 constexpr int blocks_per_sm(int elements) { return elements <= 4 ? 4 : 3; }
 
 // How [n][width] gradients are cut: C vectors of `lanes` lanes in a group,
@@ -52,20 +55,26 @@ struct Cut {
   int64_t slices, blocks;
 };
 
+// Whether a cut that covers `padded` columns wastes little beside `least`.
+inline bool close_to(int64_t padded, int64_t least) { return padded * 8 <= least * 9; }
+
 // Lanes of a group for rows of `vectors` vectors, C a lane: a short row whole;
-// else the width from 4 lanes (which read 64 bytes side by side) to 32 that
-// leaves the fewest lanes without a column. `padded` is what it covers.
+// else the most, from 32 down to four (which read 64 bytes side by side), that
+// leave few lanes without a column. `padded` is what they cover.
 inline int lanes_of(int64_t vectors, int c, int64_t* padded) {
-  int best = 1;
-  while (best < 4 && best * c < vectors) best *= 2;
-  *padded = (vectors + best * c - 1) / (best * c) * (best * c);
-  if (best < 4) return best;
-  *padded = INT64_MAX;
-  for (int lanes = 32; lanes >= 4; lanes /= 2) {
-    const int64_t covered = (vectors + lanes * c - 1) / (lanes * c) * (lanes * c);
-    if (covered < *padded) *padded = covered, best = lanes;
+  auto covered = [&](int lanes) {
+    return (vectors + lanes * c - 1) / (lanes * c) * (lanes * c);
+  };
+  int lanes = 1;
+  while (lanes < 4 && lanes * c < vectors) lanes *= 2;
+  if (lanes == 4) {
+    const int64_t least = std::min(std::min(covered(4), covered(8)),
+                                   std::min(covered(16), covered(32)));
+    lanes = 32;
+    while (!close_to(covered(lanes), least)) lanes /= 2;
   }
-  return best;
+  *padded = covered(lanes);
+  return lanes;
 }
 
 inline Cut cut_of(int64_t n, int64_t width, int vec, int c, int64_t rest) {
@@ -230,8 +239,10 @@ inline int64_t rest_blocks(int64_t rows, int64_t width, int vec) {
 enum Head : unsigned char { kNone = 0, kEnded = 1, kOpen = 2 };
 
 // V: elements of a vector of gradients, C: vectors of a lane, R: elements of a
-// vector of the rows without tokens.
-template <class T, int V, int C, int R, bool kDrop, class End>
+// vector of the rows without tokens. kLoose: vectors of four elements that may
+// begin anywhere and end behind the row, moved one by one (for dropout on odd
+// rows: single elements would draw four words for every one they use).
+template <class T, int V, int C, int R, bool kDrop, bool kLoose, class End>
 __global__ void __launch_bounds__(kThreads, blocks_per_sm(C * V))
     sum_kernel(const __grid_constant__ Args<T> a, const End end) {
   wait_before();
@@ -253,9 +264,13 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(C * V))
   // This lane's columns: `column` and C - 1 more, `apart` from each other.
   const int apart = a.cut.lanes * V;
   const int64_t column = (job - block * a.cut.slices) * (apart * C) + lane * V;
-  bool live[C];
+  // How many elements of each vector there are (all or none unless kLoose).
+  int live[C];
 #pragma unroll
-  for (int c = 0; c < C; ++c) live[c] = column + c * apart < a.width;
+  for (int c = 0; c < C; ++c) {
+    const int64_t left = a.width - column - c * apart;
+    live[c] = left >= V ? V : left > 0 ? int(left) : 0;
+  }
   const int64_t first = block * a.cut.block;
   const int count = int(a.n - first < a.cut.block ? a.n - first : a.cut.block);
   // Entries of the block and one on each side (kNoRow past the list's ends).
@@ -289,7 +304,13 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(C * V))
     for (int c = 0; c < C; ++c)
       if (live[c]) {
         scale<V>(sum[c], a.factor);
-        end.template put<V>(at + c * apart, sum[c]);
+        if constexpr (kLoose) {
+#pragma unroll
+          for (int j = 0; j < V; ++j)
+            if (j < live[c]) end.template put<1>(at + c * apart + j, {sum[c][j]});
+        } else {
+          end.template put<V>(at + c * apart, sum[c]);
+        }
       }
   };
   auto put_head = [&] {
@@ -304,8 +325,9 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(C * V))
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       bool keep[V];
-      if constexpr (kDrop)
-        mask_vector<V>(a.mask, offset, uint64_t(position * a.width + column + c * apart), keep);
+      const uint64_t element = uint64_t(position * a.width + column + c * apart);
+      if constexpr (kDrop && kLoose) mask_four(a.mask, offset, element, keep);
+      else if constexpr (kDrop) mask_vector<V>(a.mask, offset, element, keep);
 #pragma unroll
       for (int j = 0; j < V; ++j)
         sum[c][j] += !kDrop || keep[j] ? to_float(g[c].v[j]) : 0.f;
@@ -313,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(C * V))
   };
 
   const T* grad = a.grad + column;
-  constexpr int U = rows_at_once(C);
+  constexpr int U = rows_at_once(C * V * sizeof(T), kLoose);
   for (int i = begin; i < stop; i += U) {
     uint2 token[U];
     Vec<T, V> g[U][C];
@@ -324,7 +346,13 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(C * V))
         const T* from = grad + token[u].y * a.stride;
 #pragma unroll
         for (int c = 0; c < C; ++c)
-          if (live[c]) g[u][c] = read_once<T, V>(from + c * apart);
+          if constexpr (kLoose) {
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+              if (j < live[c]) g[u][c].v[j] = from[c * apart + j];
+          } else if (live[c]) {
+            g[u][c] = read_once<T, V>(from + c * apart);
+          }
       }
     if (i + U <= stop && token[U - 1].x == row) {  // all of one row, which is the current one
 #pragma unroll
@@ -376,7 +404,16 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(C * V))
   auto put_partial = [&](int64_t which) {
 #pragma unroll
     for (int c = 0; c < C; ++c)
-      if (live[c]) put<V>(a.partial + which * a.width + column + c * apart, sum[c]);
+      if (live[c]) {
+        float* to = a.partial + which * a.width + column + c * apart;
+        if constexpr (kLoose) {
+#pragma unroll
+          for (int j = 0; j < V; ++j)
+            if (j < live[c]) to[j] = sum[c][j];
+        } else {
+          put<V>(to, sum[c]);
+        }
+      }
   };
   if (continued) {
     if (join(group + 1)) put_partial(2 * block + 1);
@@ -502,9 +539,8 @@ __global__ void __launch_bounds__(kThreads)
 // ---- host ----
 
 // Vectors of a lane: one, three or four floats' vectors, one or two of 16-bit
-// elements (16 running sums a lane at most), whatever covers a row with the
-// fewest idle lanes; more of them where that is equal, unless the rows are so
-// few that the groups would not fill the GPU.
+// elements (16 running sums a lane at most): the most that leave few lanes
+// idle, unless the rows are so few that the groups would not fill the GPU.
 inline int vectors_of_lane(int64_t n, int64_t width, int vec, bool floats) {
   const int64_t vectors = (width + vec - 1) / vec;
   const int more = floats ? 4 : 2, other = floats ? 3 : 1;
@@ -514,36 +550,44 @@ inline int vectors_of_lane(int64_t n, int64_t width, int vec, bool floats) {
   lanes_of(vectors, more, &most);
   const int64_t least = std::min(one, std::min(some, most));
   auto fills = [&](int c, int64_t padded) {
-    return padded == least && n * (padded / c) >= int64_t(kSms) * 512 * kLeastTokens;
+    return close_to(padded, least) && n * (padded / c) >= int64_t(kSms) * 512 * kLeastTokens;
   };
   if (fills(more, most)) return more;
   return fills(other, some) ? other : 1;
 }
 
-template <class T, int V, int C, int R, class End>
-cudaError_t run_cut(Args<T> a, const End& end, bool drop, cudaStream_t stream) {
+template <class T, int V, int C, int R, bool kDrop, bool kLoose, class End>
+cudaError_t run_cut(Args<T> a, const End& end, cudaStream_t stream) {
   a.rest = End::kRest ? rest_blocks(a.rows, a.width, R) : 0;
   a.cut = cut_of(a.n, a.width, V, C, a.rest);
   const unsigned grid = unsigned(a.rest + a.cut.blocks * a.cut.slices);
-  auto* kernel = drop ? sum_kernel<T, V, C, R, true, End> : sum_kernel<T, V, C, R, false, End>;
-  const cudaError_t e = launch_after(kernel, grid, kThreads, 0, stream, a, end);
+  const cudaError_t e = launch_after(sum_kernel<T, V, C, R, kDrop, kLoose, End>, grid, kThreads, 0,
+                                     stream, a, end);
   if (e != cudaSuccess || a.cut.blocks == 1) return e;
+  constexpr int J = kLoose ? 1 : V;
   int64_t padded;
-  const int lanes = lanes_of((a.width + V - 1) / V, 1, &padded);
-  return launch_after(join_kernel<T, V, End>, unsigned(a.cut.blocks * (padded / lanes)), kThreads,
+  const int lanes = lanes_of((a.width + J - 1) / J, 1, &padded);
+  return launch_after(join_kernel<T, J, End>, unsigned(a.cut.blocks * (padded / lanes)), kThreads,
                       0, stream, a, lanes, padded / lanes, end);
+}
+
+template <class T, int V, int R, bool kDrop, class End>
+cudaError_t run_vectors(const Args<T>& a, const End& end, cudaStream_t stream) {
+  constexpr bool kFloats = sizeof(T) == 4;
+  const int c = vectors_of_lane(a.n, a.width, V, kFloats);
+  if (c == 1) return run_cut<T, V, 1, R, kDrop, false, End>(a, end, stream);
+  if constexpr (kFloats)
+    return c == 3 ? run_cut<T, V, 3, R, kDrop, false, End>(a, end, stream)
+                  : run_cut<T, V, 4, R, kDrop, false, End>(a, end, stream);
+  else
+    return run_cut<T, V, 2, R, kDrop, false, End>(a, end, stream);
 }
 
 template <class T, int V, int R, class End>
 cudaError_t run_sums(const Args<T>& a, const End& end, bool drop, cudaStream_t stream) {
-  constexpr bool kFloats = sizeof(T) == 4;
-  const int c = vectors_of_lane(a.n, a.width, V, kFloats);
-  if (c == 1) return run_cut<T, V, 1, R, End>(a, end, drop, stream);
-  if constexpr (kFloats)
-    return c == 3 ? run_cut<T, V, 3, R, End>(a, end, drop, stream)
-                  : run_cut<T, V, 4, R, End>(a, end, drop, stream);
-  else
-    return run_cut<T, V, 2, R, End>(a, end, drop, stream);
+  if (!drop) return run_vectors<T, V, R, false, End>(a, end, stream);
+  if constexpr (V == 1) return run_cut<T, 4, 1, R, true, true, End>(a, end, stream);
+  else return run_vectors<T, V, R, true, End>(a, end, stream);
 }
 
 template <class T>

@@ -36,8 +36,7 @@ from typing import NamedTuple
 import torch
 
 import _native as native
-from consume import check_disjoint
-from dropout import TYPES, check_draw, launch, overlap
+from dropout import TYPES, check_draw, launch
 
 MOST = 2 ** 31 - 1
 _BITS = {torch.int32: 32, torch.int64: 64}
@@ -84,8 +83,8 @@ def _matrix(t, name):
     """t as a matrix with unit column stride: (tensor, type, rows, width, row
     stride)."""
     kind = TYPES.get(t.dtype)
-    _require(t.is_cuda and kind is not None, f"{name} must be CUDA float32, float16 or bfloat16")
-    _require(t.dim() == 2, f"{name} must be a matrix")
+    if not (t.is_cuda and kind is not None and t.dim() == 2):
+        raise RuntimeError(f"{name} must be a CUDA matrix of float32, float16 or bfloat16")
     rows, width = t.shape
     if t.is_contiguous():
         return t, kind, rows, width, width
@@ -133,9 +132,10 @@ def _tokens(index, rows, padding_index, order, count, device):
     return (None, 0, 0, 0, native.ptr(order.pairs)), order.pairs
 
 
-def _workspace(count, rows, width, consume, ordered, device):
+def _workspace(count, rows, width, consume, ordered, like):
+    """A call's workspace as a tensor: (tensor, bytes)."""
     need = native.library().clad3dgs_embedding_workspace(count, rows, width, consume, ordered)
-    return torch.empty(need, dtype=torch.uint8, device=device), need
+    return like.new_empty(need, dtype=torch.uint8), need
 
 
 def _lookup(table, index, scale, padding_index, p, seed, offset):
@@ -168,10 +168,10 @@ def lookup_gradient(grad, index, rows, *, scale=1.0, padding_index=None, p=0.0, 
     tokens, alive = _tokens(index, rows, padding_index, order, count, device)
     out = grad.new_empty((rows, width))
     if out.numel():
-        workspace, need = _workspace(count, rows, width, 0, order is not None, device)
+        workspace, need = _workspace(count, rows, width, 0, order is not None, out)
         launch(device, "embedding gradient", native.library().clad3dgs_embedding_gradient, kind,
-               count, rows, width, native.ptr(grad), stride, *tokens, scale, p, seed, number,
-               address, out.data_ptr(), native.ptr(workspace), need)
+               count, rows, width, grad.data_ptr(), stride, *tokens, scale, p, seed, number,
+               address, out.data_ptr(), workspace.data_ptr(), need)
     return out
 
 
@@ -185,27 +185,35 @@ def consume_torch_adam(table, first, second, grad, index, *, rate, bias1, bias2_
     grad, kind, count, width, stride = _gradient_matrix(grad)
     device = grad.device
     _require(table.dim() == 2, "table must be a matrix")
-    rows = table.shape[0]
-    for name, t in (("table", table), ("first", first), ("second", second)):
-        _require(t.dtype == torch.float32 and t.device == device and t.shape == (rows, width)
-                 and t.is_contiguous(),
-                 f"{name} must be contiguous CUDA float32 [rows, width] on grad's device")
+    state = (table, first, second)
+    shape = table.shape
+    rows = shape[0]
+    for t in state:
+        _require(t.dtype == torch.float32 and t.device == device and t.shape == shape
+                 and t.is_contiguous(), "table and moments must be contiguous CUDA float32 "
+                 "[rows, width] on grad's device")
+    _require(shape[1] == width, "table and grad must have the same width")
     _check_rows(rows)
     _check_scale(scale)
     _require(math.isfinite(rate) and rate >= 0 and 0 < bias1 <= 1 and 0 < bias2_sqrt <= 1,
              "invalid Adam configuration")
     number, address = check_draw(p, seed, offset, device)
     tokens, alive = _tokens(index, rows, padding_index, order, count, device)
-    check_disjoint([table, first, second], [alive],
-                   "table, moments and indices must be disjoint")
-    _require(not any(overlap(grad, t) for t in (table, first, second)),
-             "table, moments and gradient must be disjoint")
-    if table.numel():
-        workspace, need = _workspace(count, rows, width, 1, order is not None, device)
+    size = 4 * rows * width
+    spans = [(t.data_ptr(), t.data_ptr() + size) for t in state]
+    read = [(grad.data_ptr(), grad.data_ptr()
+             + ((count - 1) * stride + width) * grad.element_size()),
+            (alive.data_ptr(), alive.data_ptr() + alive.numel() * alive.element_size())
+            ] if count else []
+    _require(not size or not any(
+        a < d and c < b for k, (a, b) in enumerate(spans) for c, d in spans[k + 1:] + read),
+        "table, moments, gradient and indices must be disjoint")
+    if size:
+        workspace, need = _workspace(count, rows, width, 1, order is not None, table)
         launch(device, "embedding consume", native.library().clad3dgs_embedding_consume_torch_adam,
-               kind, count, rows, width, native.ptr(grad), stride, *tokens, scale, p, seed, number,
-               address, table.data_ptr(), first.data_ptr(), second.data_ptr(), rate,
-               native.TorchAdamConfig(bias1, bias2_sqrt), native.ptr(workspace), need)
+               kind, count, rows, width, grad.data_ptr(), stride, *tokens, scale, p, seed, number,
+               address, spans[0][0], spans[1][0], spans[2][0], rate,
+               native.TorchAdamConfig(bias1, bias2_sqrt), workspace.data_ptr(), need)
 
 
 class _Lookup(torch.autograd.Function):
