@@ -264,6 +264,7 @@ struct Tokens {
     if (uint64_t(workspace) % 256 || uint64_t(order) % 8) return "unaligned workspace or order";
     return nullptr;
   }
+  float* partial() const { return reinterpret_cast<float*>(workspace + order_bytes()); }
   // The arguments of the sums; sorts first where it has to.
   template <class T>
   cudaError_t prepare(sums::Args<T>* a, const void* grad, int64_t stride,
@@ -276,7 +277,7 @@ struct Tokens {
     a->order = reinterpret_cast<const uint2*>(order);
     a->factor = factor;
     a->mask = mask;
-    a->partial = reinterpret_cast<float*>(workspace + order_bytes());
+    a->partial = partial();
     if (order || n == 0) return cudaSuccess;
     uint2* sorted = reinterpret_cast<uint2*>(workspace);
     a->order = sorted;
@@ -394,8 +395,10 @@ extern "C" int clad3dgs_embedding_consume_torch_adam(
   auto go = [&](auto zero) {
     using T = decltype(zero);
     sums::Args<T> a{};
-    const cudaError_t e =
-        tokens.prepare(&a, grad, grad_stride, mask, factor_of(scale, p), stream);
+    cudaError_t e = n > 0 ? sums::Kept(tokens.partial(), n, rows, width).clear(rows, stream)
+                          : cudaSuccess;
+    if (e == cudaSuccess)
+      e = tokens.prepare(&a, grad, grad_stride, mask, factor_of(scale, p), stream);
     return e == cudaSuccess ? sums::consume(a, adam, p > 0.0, stream) : e;
   };
   return status(what, type == CLAD3DGS_F32   ? go(float())

@@ -273,10 +273,14 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(C * V))
   }
   const int64_t first = block * a.cut.block;
   const int count = int(a.n - first < a.cut.block ? a.n - first : a.cut.block);
-  // Entries of the block and one on each side (kNoRow past the list's ends).
+  // Entries of the block and one on each side (kNoRow past the list's ends). A
+  // list that no sort has made must not lead anywhere else: positions are held
+  // in range here, rows where sums are handed on.
   for (int i = threadIdx.x; i < count + 2; i += kThreads) {
     const int64_t at = first + i - 1;
-    entries[i] = at >= 0 && at < a.n ? a.order[at] : make_uint2(kNoRow, 0);
+    uint2 one = at >= 0 && at < a.n ? a.order[at] : make_uint2(kNoRow, 0);
+    if (one.y >= a.n) one.y = 0;
+    entries[i] = one;
   }
   __syncthreads();
   const uint2* entry = entries + 1;
@@ -299,6 +303,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(C * V))
   };
   uint32_t row = begin < stop ? entry[begin].x : kNoRow;
   auto done = [&](int i) {  // i: a token of the row
+    if (row >= a.rows) return;
     const int64_t at = end.place(row, first + i, column) * a.width + column;
 #pragma unroll
     for (int c = 0; c < C; ++c)
@@ -642,20 +647,31 @@ cudaError_t run_adam(int64_t rows, int64_t width, const int32_t* slots, const fl
                       adam);
 }
 
+// Where the Adam pass finds the sums: behind the partial ones in the workspace.
+struct Kept {
+  int32_t* slots;
+  float* sums;
+
+  Kept(float* partial, int64_t n, int64_t rows, int64_t width) {
+    char* at = reinterpret_cast<char*>(partial) + gradient_bytes(n, width);
+    slots = reinterpret_cast<int32_t*>(at);
+    sums = reinterpret_cast<float*>(at + slot_bytes(rows));
+  }
+  // No row has a slot. Comes first of a call's work: in between it would keep
+  // the kernels behind it from starting early.
+  cudaError_t clear(int64_t rows, cudaStream_t stream) const {
+    return cudaMemsetAsync(slots, 0, size_t(rows) * sizeof(int32_t), stream);
+  }
+};
+
 template <class T>
 cudaError_t consume(const Args<T>& a, const Adam& adam, bool drop, cudaStream_t stream) {
   constexpr int V = 16 / sizeof(T);
-  int32_t* slots = nullptr;
-  float* kept = nullptr;
+  const Kept kept(a.partial, a.n, a.rows, a.width);
   if (a.n > 0) {
-    char* at = reinterpret_cast<char*>(a.partial) + gradient_bytes(a.n, a.width);
-    slots = reinterpret_cast<int32_t*>(at);
-    kept = reinterpret_cast<float*>(at + slot_bytes(a.rows));
-    cudaError_t e = cudaMemsetAsync(slots, 0, size_t(a.rows) * sizeof(int32_t), stream);
-    if (e != cudaSuccess) return e;
-    const Keep end{kept, slots, a.rows <= a.n};
-    e = aligned(a) ? run_sums<T, V, 1>(a, end, drop, stream)
-                   : run_sums<T, 1, 1>(a, end, drop, stream);
+    const Keep end{kept.sums, kept.slots, a.rows <= a.n};
+    const cudaError_t e = aligned(a) ? run_sums<T, V, 1>(a, end, drop, stream)
+                                     : run_sums<T, 1, 1>(a, end, drop, stream);
     if (e != cudaSuccess) return e;
   }
   const bool whole = common_bytes(uint64_t(a.width * sizeof(float)) | uint64_t(adam.table) |
@@ -663,7 +679,7 @@ cudaError_t consume(const Args<T>& a, const Adam& adam, bool drop, cudaStream_t 
   const bool narrow = Narrow::fits(a.rows * a.width + 2 * kThreads);
   auto* run = whole ? (narrow ? run_adam<Narrow, 4> : run_adam<Wide, 4>)
                     : (narrow ? run_adam<Narrow, 1> : run_adam<Wide, 1>);
-  return run(a.rows, a.width, slots, kept, adam, stream);
+  return run(a.rows, a.width, a.n > 0 ? kept.slots : nullptr, kept.sums, adam, stream);
 }
 
 }  // namespace sums

@@ -126,10 +126,11 @@ def _tokens(index, rows, padding_index, order, count, device):
         index, bits = _index(index, device)
         _require(index.numel() == count, "grad must have one row per token")
         return (native.ptr(index), bits, *_padding(padding_index), None), index
-    _require(isinstance(order, TokenOrder) and order.rows == rows
-             and order.pairs.shape[0] == count and order.pairs.device == device,
+    pairs = order.pairs if isinstance(order, TokenOrder) else None
+    _require(pairs is not None and order.rows == rows and pairs.shape == (count, 2)
+             and pairs.device == device and pairs.dtype == torch.int32 and pairs.is_contiguous(),
              "the token order belongs to another table, device or number of tokens")
-    return (None, 0, 0, 0, native.ptr(order.pairs)), order.pairs
+    return (None, 0, 0, 0, native.ptr(pairs)), pairs
 
 
 def _workspace(count, rows, width, consume, ordered, like):

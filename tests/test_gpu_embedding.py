@@ -240,6 +240,26 @@ def test_infinities_and_nan_stay_where_they_are(cuda):
     assert np.array_equal(torch.isnan(got).cpu().numpy(), kept) and not got.nan_to_num().any()
 
 
+def test_an_order_that_no_sort_made_stays_in_bounds(cuda):
+    """A TokenOrder is an ordinary tensor: whatever it holds, nothing outside the
+    gradient and the table is touched (what comes out is then anything)."""
+    import embedding
+
+    rows, width, n = 40, 48, 5000
+    _, index, grad = _case(n, rows, width, torch.float32, cuda)
+    room = torch.full((rows + 200, width), 7.0, device=cuda)  # the table lies inside
+    state = [room[100:100 + rows], *(_adam_state(rows, width, cuda)[1:])]
+    rng = np.random.default_rng(0)
+    for pairs in (rng.integers(-2 ** 31, 2 ** 31, (n, 2)), rng.integers(0, 100, (n, 2)),
+                  np.stack([rng.integers(0, 60, n), rng.integers(0, 2 * n, n)], axis=1)):
+        order = embedding.TokenOrder(torch.from_numpy(pairs.astype(np.int32)).to(cuda), rows)
+        embedding.lookup_gradient(grad, None, rows, order=order)
+        embedding.consume_torch_adam(*state, grad, None, rate=0.1, bias1=0.5, bias2_sqrt=0.5,
+                                     order=order)
+        torch.cuda.synchronize()
+        assert (room[:100] == 7).all() and (room[100 + rows:] == 7).all()
+
+
 def test_far_rows(cuda):
     """Element offsets past 2^32 in the table and in its gradient."""
     import embedding
@@ -453,6 +473,11 @@ def test_refusals(cuda):
         lambda: embedding.lookup_gradient(grad, index, -1),
         lambda: embedding.lookup_gradient(grad, None, 5, order=order),
         lambda: embedding.lookup_gradient(grad[:9], None, 4, order=order),
+        lambda: embedding.lookup_gradient(grad, None, 4, order=order._replace(
+            pairs=order.pairs.long())),
+        lambda: embedding.lookup_gradient(grad, None, 4, order=order._replace(
+            pairs=order.pairs.t().contiguous().t())),
+        lambda: embedding.lookup_gradient(grad, None, 4, order=order.pairs),
         lambda: embedding.lookup_gradient(grad.double(), index, 4),
         lambda: embedding.lookup_gradient(grad, index, 4, seed=-1),
         lambda: embedding.consume_torch_adam(*state, grad[:, :5], index, **adam),
@@ -513,3 +538,24 @@ def test_lookup_feeds_the_renderer(cuda):
         embedding.consume_torch_adam(codebook, first, second, h.view(n, 48), index, rate=0.0025,
                                      bias1=0.1, bias2_sqrt=math.sqrt(0.001))
     assert (codebook.detach() - before).abs().max() <= 0.0026 and (first != 0).any()
+
+
+@pytest.mark.parametrize("dtype,n,rows,width", [(torch.float16, 300, 40_000, 1024),
+                                                (torch.float32, 20_000, 131_072, 160),
+                                                (torch.bfloat16, 3, 9_000_001, 8)])
+def test_large_table_of_which_few_rows_are_named(cuda, dtype, n, rows, width):
+    """64 MiB of gradient and more, most rows without a token: an uninitialised
+    output is zero everywhere else."""
+    import embedding
+
+    _, index, grad = _case(n, 1000, width, dtype, cuda, kind="uniform", padding=True)
+    index = torch.where(index >= 0, index * (rows // 1000), index)
+    torch.full((rows, width), float("nan"), dtype=dtype, device=cuda)  # what the memory held
+    got = embedding.lookup_gradient(grad, index, rows, padding_index=-1)
+    named = index[index >= 0].unique()
+    few = torch.full((rows,), -1, device=cuda)
+    few[named] = torch.arange(len(named), device=cuda)
+    _check_gradient(got[named], grad, torch.where(index >= 0, few[index.clamp(min=0)], -1),
+                    len(named), 1.0, 0.0, dtype)
+    got[named] = 0
+    assert not got.any() and not torch.isnan(got).any()
