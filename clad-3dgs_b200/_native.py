@@ -193,12 +193,24 @@ def stream_handle(stream=None) -> int:
     return s.cuda_stream
 
 
+def current_device() -> int:
+    """torch.cuda.current_device() without its check that CUDA is initialised
+    (whoever holds a CUDA tensor has done that)."""
+    import torch
+
+    global current_device
+    current_device = torch._C._cuda_getDevice
+    return current_device()
+
+
 def raw_stream(device_index: int) -> int:
     """The current stream of a device, as stream_handle gives it, without making
     a Stream object (0.1 us instead of 3)."""
-    from torch._C import _cuda_getCurrentRawStream
+    import torch
 
-    return _cuda_getCurrentRawStream(device_index)
+    global raw_stream
+    raw_stream = torch._C._cuda_getCurrentRawStream
+    return raw_stream(device_index)
 
 
 def fault_status(clear: bool = True) -> int:

@@ -58,7 +58,9 @@ __device__ __forceinline__ Vec<T, V> finish(const Vec<T, V>& x, const bool (&kee
 // A lookup is bound by writing its output (the index and the table's rows come on
 // top; small tables stay in L2). Threads take consecutive vectors of 16 bytes of
 // the output, whatever rows they belong to, so that stores are whole lines, U of
-// them each, all asked for before the first is stored.
+// them each, all asked for before the first is stored. 1.1M rows of 48 floats
+// from 4096: 40 us (5.3 TB/s; groups of lanes a row 50, one vector a thread
+// 147); 16384 of 2048 bf16 from 131072: 23 us (5.8 TB/s).
 template <class T, class Division, int V, int U, bool kDrop>
 __global__ void __launch_bounds__(kThreads)
     lookup_kernel(typename Division::Number total, const Division vectors,
@@ -99,7 +101,9 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // Rows that do not start on 16 bytes: V consecutive elements of the output a
-// thread from single loads (neighbours hit the same lines). A vector touches
+// thread from single loads (neighbours hit the same lines); bound by their
+// instructions (100003 x 77 f16 with dropout: 14 us, the call's launch included,
+// against 98 with one element a thread). A vector touches
 // two rows at most, or any number of rows shorter than itself (kShort).
 template <class T, class Division, int V, bool kShort, bool kDrop>
 __global__ void __launch_bounds__(kThreads)

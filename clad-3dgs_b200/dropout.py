@@ -64,7 +64,7 @@ def row_layout(x):
 def launch(device, what, entry, *arguments):
     """Calls a C entry on the current stream of `device`, with it current."""
     index = device.index
-    if index == torch.cuda.current_device():
+    if index == native.current_device():
         status = entry(*arguments, native.raw_stream(index))
     else:
         with torch.cuda.device(device):

@@ -31,6 +31,7 @@ written.
 from __future__ import annotations
 
 import math
+from functools import lru_cache
 from typing import NamedTuple
 
 import torch
@@ -133,9 +134,14 @@ def _tokens(index, rows, padding_index, order, count, device):
     return (None, 0, 0, 0, native.ptr(pairs)), pairs
 
 
+@lru_cache(maxsize=4096)
+def _workspace_bytes(count, rows, width, consume, ordered):
+    return native.library().clad3dgs_embedding_workspace(count, rows, width, consume, ordered)
+
+
 def _workspace(count, rows, width, consume, ordered, like):
     """A call's workspace as a tensor: (tensor, bytes)."""
-    need = native.library().clad3dgs_embedding_workspace(count, rows, width, consume, ordered)
+    need = _workspace_bytes(count, rows, width, consume, ordered)
     return like.new_empty(need, dtype=torch.uint8), need
 
 
