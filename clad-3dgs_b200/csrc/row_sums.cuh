@@ -17,8 +17,8 @@
 // lane share the loop's instructions, which else cost as much time as the
 // memory does. 1.1M rows of 48 floats over 8192 table rows: 45 us (4.7 TB/s; 38
 // with the rows in order, so that random rows cost 7) and 5 us for the second
-// kernel. One wave of long blocks is best: 53 us with two waves, 63 with four,
-// 56 with four blocks an SM instead of three.
+// kernel, 48 for both in a row. One wave of long blocks is best: 53 us with two
+// waves, 63 with four, 56 with four blocks an SM instead of three.
 //
 // Adam is a pass of its own over the table, because an update inside the walk
 // would wait for three loads at the end of every row (a walk over 8192 short

@@ -14,7 +14,7 @@
 // the other blocks' counts itself (they lie in L2) and scatters its share tile
 // by tile. Bound by latency at these sizes: everything a thread reads of a tile
 // is asked for before any of it is used. 16384 tokens over 131072 rows: 14 us
-// (one block took 37, four kernels over small tiles 61); 1.1M tokens over 4096
+// (one block took 37, six kernels over four tiles 66); 1.1M tokens over 4096
 // rows, two passes: 33 us, of which counting 5.5 + 4 and scattering 16 + 12,
 // half of that the launches, loads and barriers and a quarter each the ranks
 // and the scattered stores.
