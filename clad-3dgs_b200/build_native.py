@@ -14,6 +14,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
@@ -38,6 +39,9 @@ FLAGS = {
     "train_step.cu": ["-fmad=false"],
     "dropout.cu": [],
     "embedding.cu": [],
+    "row_sums_f32.cu": [],
+    "row_sums_f16.cu": [],
+    "row_sums_bf16.cu": [],
 }
 
 
@@ -59,7 +63,7 @@ def build(verbose: bool = False, ptxas_info: bool = False) -> Path:
     """Compiles every csrc/*.cu and links the shared library; returns its path."""
     BUILD.mkdir(parents=True, exist_ok=True)
     headers = sorted(CSRC.glob("*.cuh")) + sorted(INCLUDE.glob("*.h"))
-    objects = []
+    objects, commands = [], []
     for name, extra in FLAGS.items():
         source = CSRC / name
         obj = BUILD / (source.stem + ".o")
@@ -71,7 +75,9 @@ def build(verbose: bool = False, ptxas_info: bool = False) -> Path:
             cmd.insert(1, "-Xptxas=-v")
         if verbose:
             print(" ".join(cmd), flush=True)
-        subprocess.run(cmd, check=True)
+        commands.append(cmd)
+    with ThreadPoolExecutor(os.cpu_count() or 1) as pool:
+        list(pool.map(lambda cmd: subprocess.run(cmd, check=True), commands))
     if _stale(LIBRARY, objects):
         cmd = [nvcc(), *ARCH, "-shared", "-o", str(LIBRARY), *map(str, objects)]
         if verbose:

@@ -28,6 +28,12 @@
 namespace clad3dgs {
 int fail(int code, const std::string& message);  // gaussian_step.cu
 
+namespace sums {
+CLAD3DGS_ROW_SUMS(extern, float)           // row_sums_f32.cu
+CLAD3DGS_ROW_SUMS(extern, __half)          // row_sums_f16.cu
+CLAD3DGS_ROW_SUMS(extern, __nv_bfloat16)   // row_sums_bf16.cu
+}  // namespace sums
+
 // Reads (and clears) the word set by indices outside their table.
 cudaError_t token_fault(bool clear, unsigned* word) {
   cudaError_t e = cudaMemcpyFromSymbol(word, tokens::g_token_fault, sizeof(*word));
@@ -221,6 +227,8 @@ int status(const char* what, cudaError_t e) {
 
 constexpr int64_t kMostTokens = (int64_t(1) << 31) - 1;  // positions and rows are 32-bit
 
+float factor_of(double scale, double p) { return p < 1.0 ? float(scale / (1.0 - p)) : 0.f; }
+
 // The checks every entry shares; null if they pass.
 const char* problem(int64_t n, int64_t rows, int64_t width, int type, double scale, double p) {
   if (n < 0 || rows < 0 || width < 0) return "negative size";
@@ -228,12 +236,11 @@ const char* problem(int64_t n, int64_t rows, int64_t width, int type, double sca
   if (width > 0 && (n > (int64_t(1) << 60) / width || rows > (int64_t(1) << 60) / width))
     return "too many elements";
   if (type < CLAD3DGS_F32 || type > CLAD3DGS_BF16) return "unknown element type";
-  if (!std::isfinite(scale)) return "scale must be finite";
   if (!(p >= 0.0 && p <= 1.0)) return "p must lie in [0, 1]";
+  if (!std::isfinite(scale) || !std::isfinite(factor_of(scale, p)))
+    return "scale / (1 - p) must be finite in 32 bits";
   return nullptr;
 }
-
-float factor_of(double scale, double p) { return p < 1.0 ? float(scale / (1.0 - p)) : 0.f; }
 
 size_t round_up(size_t bytes) { return (bytes + 255) / 256 * 256; }
 

@@ -685,5 +685,10 @@ cudaError_t consume(const Args<T>& a, const Adam& adam, bool drop, cudaStream_t 
   return run(a.rows, a.width, a.n > 0 ? kept.slots : nullptr, kept.sums, adam, stream);
 }
 
+// The kernels of each element type are compiled in a file of their own.
+#define CLAD3DGS_ROW_SUMS(prefix, T)                                                      \
+  prefix template cudaError_t gradient<T>(const Args<T>&, T*, bool, cudaStream_t);        \
+  prefix template cudaError_t consume<T>(const Args<T>&, const Adam&, bool, cudaStream_t);
+
 }  // namespace sums
 }  // namespace clad3dgs

@@ -73,7 +73,7 @@ def _padding(padding_index):
 
 
 def _check_scale(scale):
-    _require(isinstance(scale, (int, float)) and math.isfinite(scale), "scale must be finite")
+    _require(isinstance(scale, (int, float)) and abs(scale) <= 1e38, "scale must be finite")
 
 
 def _check_rows(rows):

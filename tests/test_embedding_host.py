@@ -41,7 +41,7 @@ def _adam():
 
 
 SHARED = [dict(n=-1), dict(rows=-1), dict(n=2 ** 31), dict(rows=2 ** 31)]
-SIZED = SHARED + [dict(width=-1), dict(type=3), dict(type=-1), dict(scale=INF), dict(scale=NAN),
+SIZED = SHARED + [dict(width=-1), dict(type=3), dict(type=-1), dict(scale=INF), dict(scale=NAN), dict(scale=1e39), dict(scale=1e38, p=0.999),
                   dict(p=-0.5), dict(p=1.5), dict(p=NAN), dict(n=2 ** 30, width=2 ** 40)]
 SUMS = SIZED + [dict(grad=None), dict(order=None), dict(workspace=None), dict(workspace_bytes=8),
                 dict(grad_stride=-1), dict(workspace=2064), dict(order=516),

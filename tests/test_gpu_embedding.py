@@ -559,3 +559,82 @@ def test_large_table_of_which_few_rows_are_named(cuda, dtype, n, rows, width):
                     len(named), 1.0, 0.0, dtype)
     got[named] = 0
     assert not got.any() and not torch.isnan(got).any()
+
+
+def test_one_token_without_a_dimension(cuda):
+    """An index of shape [] gives one row; its gradient is a vector."""
+    import embedding
+
+    table = torch.randn(5, 8, device=cuda, requires_grad=True)
+    y = embedding.lookup(table, torch.tensor(3, device=cuda), scale=2.0)
+    assert y.shape == (8,) and torch.equal(y, 2 * table[3])
+    (g,) = torch.autograd.grad(y, table, torch.arange(8.0, device=cuda))
+    assert g[3].tolist() == [2.0 * k for k in range(8)] and g.abs().sum() == g[3].sum()
+
+
+def test_consume_under_two_graphs(cuda):
+    """Adam steps captured twice, replayed in turn with new gradients, indices and
+    offsets: the same bits as eager calls."""
+    import embedding
+
+    n, rows, width = 3000, 70, 48
+    offset = torch.zeros(1, dtype=torch.int64, device=cuda)
+    _, index, grad = _case(n, rows, width, torch.bfloat16, cuda, kind="skewed")
+    how = dict(rate=0.01, bias1=0.5, bias2_sqrt=0.5, p=0.3, seed=SEED, offset=offset)
+    captured, eager = _adam_state(rows, width, cuda), _adam_state(rows, width, cuda)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        embedding.consume_torch_adam(*_adam_state(rows, width, cuda), grad, index, **how)
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            embedding.consume_torch_adam(*captured, grad, index, **how)
+    for step in range(4):
+        _, i, g = _case(n, rows, width, torch.bfloat16, cuda, kind="skewed", seed=step)
+        index.copy_(i)
+        grad.copy_(g)
+        offset.fill_(step + 2 ** 40)
+        graphs[step % 2].replay()
+        embedding.consume_torch_adam(*eager, grad, index, **how)
+        assert all(torch.equal(a, b) for a, b in zip(captured, eager))
+
+
+def test_two_host_threads(cuda):
+    import threading
+
+    import embedding
+
+    cases = [_case(9000, 300, 45, torch.float32, cuda, kind="skewed", seed=s) for s in range(4)]
+    want = [embedding.lookup_gradient(g, i, 300, p=0.1, seed=1) for _, i, g in cases]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(30):
+                got = embedding.lookup_gradient(cases[k][2], cases[k][1], 300, p=0.1, seed=1)
+                torch.cuda.current_stream().synchronize()
+                if not torch.equal(got, want[k]):
+                    wrong.append(k)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,rows,width", [(1000, 30, 1001), (5000, 7, 11), (65_537, 4000, 5),
+                                          (70_000, 3, 3), (9000, 800, 514)])
+def test_odd_rows_through_the_dropout(cuda, dtype, n, rows, width):
+    import embedding
+
+    table, index, grad = _case(n, rows, width, dtype, cuda, kind="skewed", bits=32, padding=True)
+    how = dict(scale=0.7, padding_index=-1, p=0.35, seed=SEED, offset=OFFSET)
+    _check_lookup(embedding.lookup(table, index, **how), table, index, 0.7, 0.35, dtype)
+    _check_gradient(embedding.lookup_gradient(grad, index, rows, **how), grad, index, rows, 0.7,
+                    0.35, dtype)
