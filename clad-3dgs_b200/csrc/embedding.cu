@@ -34,13 +34,12 @@ CLAD3DGS_ROW_SUMS(extern, __half)          // row_sums_f16.cu
 CLAD3DGS_ROW_SUMS(extern, __nv_bfloat16)   // row_sums_bf16.cu
 }  // namespace sums
 
-// Reads (and clears) the word set by indices outside their table.
+// Reads (and clears) the words set by indices outside their table.
 cudaError_t token_fault(bool clear, unsigned* word) {
-  cudaError_t e = cudaMemcpyFromSymbol(word, tokens::g_token_fault, sizeof(*word));
-  if (e == cudaSuccess && clear && *word) {
-    const unsigned zero = 0;
-    e = cudaMemcpyToSymbol(tokens::g_token_fault, &zero, sizeof(zero));
-  }
+  cudaError_t e = tokens::take_token_fault(clear, word);
+  if (e == cudaSuccess) e = sums::take_fault<float>(clear, word);
+  if (e == cudaSuccess) e = sums::take_fault<__half>(clear, word);
+  if (e == cudaSuccess) e = sums::take_fault<__nv_bfloat16>(clear, word);
   return e;
 }
 
@@ -254,14 +253,14 @@ struct Tokens {
   char* workspace;
   size_t bytes;
 
+  bool sorts() const { return !order && n > 0 && !sums::few(n, rows, width); }
   size_t order_bytes() const {
-    return order || n == 0 ? 0
-                           : round_up(size_t(n) * sizeof(uint2)) +
-                                 round_up(tokens::sort_plan(n, rows).bytes());
+    return sorts() ? round_up(size_t(n) * sizeof(uint2)) +
+                         round_up(tokens::sort_plan(n, rows).bytes())
+                   : 0;
   }
   size_t need(bool consume) const {
-    return order_bytes() +
-           (consume ? sums::consume_bytes(n, rows, width) : n > 0 ? sums::gradient_bytes(n, width) : 0);
+    return order_bytes() + sums::workspace_bytes(n, rows, width, consume);
   }
   const char* problem(const void* grad, int64_t stride, bool consume) const {
     if (n > 0 && !grad) return "null array";
@@ -289,7 +288,7 @@ struct Tokens {
     a->factor = factor;
     a->mask = mask;
     a->partial = partial();
-    if (order || n == 0) return cudaSuccess;
+    if (!sorts()) return cudaSuccess;
     uint2* sorted = reinterpret_cast<uint2*>(workspace);
     a->order = sorted;
     return tokens::sort_tokens(n, index, sorted, workspace + round_up(size_t(n) * sizeof(uint2)),
@@ -376,7 +375,7 @@ extern "C" int clad3dgs_embedding_gradient(int type, int64_t n, int64_t rows, in
     sums::Args<T> a{};
     const cudaError_t e =
         tokens.prepare(&a, grad, grad_stride, mask, factor_of(scale, p), stream);
-    return e == cudaSuccess ? sums::gradient(a, static_cast<T*>(out), p > 0.0, stream) : e;
+    return e == cudaSuccess ? sums::gradient(a, tokens.index, static_cast<T*>(out), p > 0.0, stream) : e;
   };
   return status(what, type == CLAD3DGS_F32   ? go(float())
                       : type == CLAD3DGS_F16 ? go(__half())
@@ -406,11 +405,12 @@ extern "C" int clad3dgs_embedding_consume_torch_adam(
   auto go = [&](auto zero) {
     using T = decltype(zero);
     sums::Args<T> a{};
-    cudaError_t e = n > 0 ? sums::Kept(tokens.partial(), n, rows, width).clear(rows, stream)
-                          : cudaSuccess;
+    cudaError_t e = cudaSuccess;
+    if (n > 0 && !sums::few(n, rows, width))
+      e = sums::Kept(tokens.partial(), n, rows, width).clear(rows, stream);
     if (e == cudaSuccess)
       e = tokens.prepare(&a, grad, grad_stride, mask, factor_of(scale, p), stream);
-    return e == cudaSuccess ? sums::consume(a, adam, p > 0.0, stream) : e;
+    return e == cudaSuccess ? sums::consume(a, tokens.index, adam, p > 0.0, stream) : e;
   };
   return status(what, type == CLAD3DGS_F32   ? go(float())
                       : type == CLAD3DGS_F16 ? go(__half())

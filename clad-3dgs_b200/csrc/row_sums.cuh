@@ -34,6 +34,7 @@
 #include "element_types.cuh"
 #include "gaussian_math.cuh"
 #include "launch.cuh"
+#include "token_index.cuh"
 
 namespace clad3dgs {
 namespace sums {
@@ -544,6 +545,135 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
+// ---- few tokens, small tables ----
+
+// One launch for all of it: what counts at these sizes is the host's time for
+// each launch (2.3 us) and the workspace. Every block ranks the few tokens by
+// comparing each with all, then eight lanes share the tokens of a vector of the
+// table and add up in a fixed tree. A call on 37 tokens and 1000 x 45 f32 takes
+// 11 us instead of 17, Adam of 60 x 48 with 184 tokens 13 instead of 22.
+constexpr int kFewTokens = 512;
+constexpr int64_t kSmallTable = int64_t(1) << 18;  // elements
+constexpr int kSharing = 8;
+
+inline bool few(int64_t n, int64_t rows, int64_t width) {
+  return n > 0 && n <= kFewTokens && rows * width <= kSmallTable;
+}
+
+// Adam as what becomes of a row's sums.
+struct Update {
+  Adam adam;
+
+  template <int V>
+  __device__ __forceinline__ void put(int64_t at, const float (&sum)[V]) const {
+    constexpr int W = V < 4 ? V : 4;
+#pragma unroll
+    for (int h = 0; h < V; h += W) {
+      auto* p = reinterpret_cast<Vec<float, W>*>(adam.table + at + h);
+      auto* m = reinterpret_cast<Vec<float, W>*>(adam.first + at + h);
+      auto* v = reinterpret_cast<Vec<float, W>*>(adam.second + at + h);
+      Vec<float, W> pv = *p, mv = *m, vv = *v;
+#pragma unroll
+      for (int j = 0; j < W; ++j)
+        torch_adam(pv.v[j], mv.v[j], vv.v[j], sum[h + j], adam.step, adam.inv_bias2);
+      *p = pv;
+      *m = mv;
+      *v = vv;
+    }
+  }
+};
+
+// total: vectors of the table. The tokens come from a.order if it is given, else
+// from index.
+template <class T, int V, bool kDrop, class End>
+__global__ void __launch_bounds__(kFewTokens)
+    few_kernel(const __grid_constant__ Args<T> a, const tokens::Index index, uint32_t total,
+               const Narrow vectors, const End end) {
+  wait_before();
+  __shared__ uint2 sorted[kFewTokens];
+  __shared__ uint32_t keys[kFewTokens];
+  const int n = int(a.n), me = threadIdx.x;
+  if (a.order) {
+    if (me < n) {
+      uint2 one = a.order[me];
+      if (one.y >= a.n) one.y = 0;  // see sum_kernel
+      sorted[me] = one;
+    }
+  } else {
+    const uint32_t key = me < n ? tokens::row_of(index, tokens::raw_index(index, me)) : kNoRow;
+    keys[me] = key;
+    __syncthreads();
+    if (me < n) {
+      int rank = 0;
+      for (int j = 0; j < n; ++j) rank += keys[j] < key || (keys[j] == key && j < me);
+      sorted[rank] = make_uint2(key, uint32_t(me));
+    }
+  }
+  __syncthreads();
+  const unsigned long long offset = kDrop ? mask_offset(a.mask) : 0;
+  auto before = [&](uint32_t row) {  // tokens in front of a row's
+    int low = 0, high = n;
+    while (low < high) {
+      const int middle = (low + high) / 2;
+      if (sorted[middle].x < row) low = middle + 1;
+      else high = middle;
+    }
+    return low;
+  };
+  const int share = me % kSharing;
+  constexpr uint32_t kVectors = kFewTokens / kSharing;  // of a block at once
+  for (uint32_t first = blockIdx.x * kVectors; first < total; first += gridDim.x * kVectors) {
+    const uint32_t at = first + me / kSharing;
+    const uint32_t row = vectors.quotient(at);
+    const int64_t column = int64_t(at - row * vectors.divisor) * V;
+    const bool real = at < total;
+    float sum[V];
+    clear<V>(sum);
+    const int stop = real ? before(row + 1) : 0;
+#pragma unroll 4
+    for (int i = (real ? before(row) : 0) + share; i < stop; i += kSharing) {
+      const uint32_t position = sorted[i].y;
+      const Vec<T, V> g = read_once<T, V>(a.grad + position * a.stride + column);
+      bool keep[V];
+      if constexpr (kDrop)
+        mask_vector<V>(a.mask, offset, uint64_t(position * a.width + column), keep);
+#pragma unroll
+      for (int j = 0; j < V; ++j) sum[j] += !kDrop || keep[j] ? to_float(g.v[j]) : 0.f;
+    }
+#pragma unroll
+    for (int o = 1; o < kSharing; o *= 2)
+#pragma unroll
+      for (int j = 0; j < V; ++j) sum[j] += __shfl_xor_sync(~0u, sum[j], o);
+    if (real && share == 0) {
+      scale<V>(sum, a.factor);
+      end.template put<V>(row * a.width + column, sum);
+    }
+  }
+}
+
+template <class T, int V, class End>
+cudaError_t run_few_vectors(const Args<T>& a, const tokens::Index& index, const End& end,
+                            bool drop, cudaStream_t stream) {
+  const int64_t vectors = a.width / V, total = a.rows * vectors;
+  const int64_t blocks = (total + kFewTokens / kSharing - 1) / (kFewTokens / kSharing);
+  auto* kernel = drop ? few_kernel<T, V, true, End> : few_kernel<T, V, false, End>;
+  return launch_after(kernel, unsigned(std::min<int64_t>(blocks, kSms * 3)), kFewTokens, 0, stream,
+                      a, index, uint32_t(total), Narrow(vectors), end);
+}
+
+template <class T>
+bool aligned(const Args<T>& a) {
+  return common_bytes(uint64_t(a.width * sizeof(T)) | uint64_t(a.stride * sizeof(T)) |
+                      uint64_t(a.grad)) == 16;
+}
+
+template <class T, class End>
+cudaError_t run_few(const Args<T>& a, const tokens::Index& index, const End& end, bool whole,
+                    bool drop, cudaStream_t stream) {
+  return whole && aligned(a) ? run_few_vectors<T, 16 / sizeof(T)>(a, index, end, drop, stream)
+                             : run_few_vectors<T, 1>(a, index, end, drop, stream);
+}
+
 // ---- host ----
 
 // Vectors of a lane: one, three or four floats' vectors, one or two of 16-bit
@@ -598,19 +728,15 @@ cudaError_t run_sums(const Args<T>& a, const End& end, bool drop, cudaStream_t s
   else return run_vectors<T, V, R, true, End>(a, end, stream);
 }
 
-template <class T>
-bool aligned(const Args<T>& a) {
-  return common_bytes(uint64_t(a.width * sizeof(T)) | uint64_t(a.stride * sizeof(T)) |
-                      uint64_t(a.grad)) == 16;
-}
-
 // Vectors are 16 bytes where the rows of all arrays begin on 16, else single
 // elements.
 template <class T>
-cudaError_t gradient(const Args<T>& a, T* out, bool drop, cudaStream_t stream) {
+cudaError_t gradient(const Args<T>& a, const tokens::Index& index, T* out, bool drop,
+                     cudaStream_t stream) {
   constexpr int V = 16 / sizeof(T);
   const Store<T> end{out};
   const bool whole = common_bytes(uint64_t(a.width * sizeof(T)) | uint64_t(out)) == 16;
+  if (few(a.n, a.rows, a.width)) return run_few(a, index, end, whole, drop, stream);
   if (a.n == 0) {
     auto* kernel = whole ? rest_kernel<V, Store<T>> : rest_kernel<1, Store<T>>;
     return launch_after(kernel, unsigned(rest_blocks(a.rows, a.width, whole ? V : 1)), kThreads, 0,
@@ -623,7 +749,7 @@ cudaError_t gradient(const Args<T>& a, T* out, bool drop, cudaStream_t stream) {
 
 // Workspace of the partial sums for any cut of these sizes: a group has
 // kLeastTokens at least, a block at least a group for each 32 lanes.
-inline size_t gradient_bytes(int64_t n, int64_t width) {
+inline size_t partial_bytes(int64_t n, int64_t width) {
   const int64_t least = kThreads / 32 * kLeastTokens;
   const size_t bytes = size_t(2 * ((n + least - 1) / least)) * width * sizeof(float);
   return (bytes + 15) / 16 * 16;
@@ -633,9 +759,10 @@ inline size_t gradient_bytes(int64_t n, int64_t width) {
 // name (no more than rows, nor than tokens).
 inline size_t slot_bytes(int64_t rows) { return (size_t(rows) * sizeof(int32_t) + 15) / 16 * 16; }
 
-inline size_t consume_bytes(int64_t n, int64_t rows, int64_t width) {
-  if (n == 0) return 0;
-  return gradient_bytes(n, width) + slot_bytes(rows) +
+inline size_t workspace_bytes(int64_t n, int64_t rows, int64_t width, bool consume) {
+  if (n == 0 || few(n, rows, width)) return 0;
+  if (!consume) return partial_bytes(n, width);
+  return partial_bytes(n, width) + slot_bytes(rows) +
          size_t(std::min(n, rows)) * width * sizeof(float);
 }
 
@@ -656,7 +783,7 @@ struct Kept {
   float* sums;
 
   Kept(float* partial, int64_t n, int64_t rows, int64_t width) {
-    char* at = reinterpret_cast<char*>(partial) + gradient_bytes(n, width);
+    char* at = reinterpret_cast<char*>(partial) + partial_bytes(n, width);
     slots = reinterpret_cast<int32_t*>(at);
     sums = reinterpret_cast<float*>(at + slot_bytes(rows));
   }
@@ -668,8 +795,12 @@ struct Kept {
 };
 
 template <class T>
-cudaError_t consume(const Args<T>& a, const Adam& adam, bool drop, cudaStream_t stream) {
+cudaError_t consume(const Args<T>& a, const tokens::Index& index, const Adam& adam, bool drop,
+                    cudaStream_t stream) {
   constexpr int V = 16 / sizeof(T);
+  const bool whole = common_bytes(uint64_t(a.width * sizeof(float)) | uint64_t(adam.table) |
+                                  uint64_t(adam.first) | uint64_t(adam.second)) == 16;
+  if (few(a.n, a.rows, a.width)) return run_few(a, index, Update{adam}, whole, drop, stream);
   const Kept kept(a.partial, a.n, a.rows, a.width);
   if (a.n > 0) {
     const Keep end{kept.sums, kept.slots, a.rows <= a.n};
@@ -677,18 +808,25 @@ cudaError_t consume(const Args<T>& a, const Adam& adam, bool drop, cudaStream_t 
                                      : run_sums<T, 1, 1>(a, end, drop, stream);
     if (e != cudaSuccess) return e;
   }
-  const bool whole = common_bytes(uint64_t(a.width * sizeof(float)) | uint64_t(adam.table) |
-                                  uint64_t(adam.first) | uint64_t(adam.second)) == 16;
   const bool narrow = Narrow::fits(a.rows * a.width + 2 * kThreads);
   auto* run = whole ? (narrow ? run_adam<Narrow, 4> : run_adam<Wide, 4>)
                     : (narrow ? run_adam<Narrow, 1> : run_adam<Wide, 1>);
   return run(a.rows, a.width, a.n > 0 ? kept.slots : nullptr, kept.sums, adam, stream);
 }
 
+// The fault word of the file that holds T's kernels.
+template <class T>
+cudaError_t take_fault(bool clear, unsigned* word) {
+  return tokens::take_token_fault(clear, word);
+}
+
 // The kernels of each element type are compiled in a file of their own.
 #define CLAD3DGS_ROW_SUMS(prefix, T)                                                      \
-  prefix template cudaError_t gradient<T>(const Args<T>&, T*, bool, cudaStream_t);        \
-  prefix template cudaError_t consume<T>(const Args<T>&, const Adam&, bool, cudaStream_t);
+  prefix template cudaError_t gradient<T>(const Args<T>&, const tokens::Index&, T*, bool,  \
+                                          cudaStream_t);                                   \
+  prefix template cudaError_t consume<T>(const Args<T>&, const tokens::Index&, const Adam&, \
+                                         bool, cudaStream_t);                              \
+  prefix template cudaError_t take_fault<T>(bool, unsigned*);
 
 }  // namespace sums
 }  // namespace clad3dgs

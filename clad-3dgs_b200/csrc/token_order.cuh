@@ -25,36 +25,10 @@
 #include <cstdint>
 
 #include "launch.cuh"
+#include "token_index.cuh"
 
 namespace clad3dgs {
 namespace tokens {
-
-// Set when a kernel met an index outside its table that is not the padding.
-constexpr unsigned kFaultTokenRange = 256u;
-__device__ unsigned int g_token_fault = 0;
-
-// The indices a caller gives.
-struct Index {
-  const void* data;
-  bool wide;  // int64, else int32
-  bool has_padding;
-  int64_t padding;
-  int64_t rows;
-};
-
-__device__ __forceinline__ int64_t raw_index(const Index& x, int64_t i) {
-  return x.wide ? static_cast<const int64_t*>(x.data)[i]
-                : int64_t(static_cast<const int32_t*>(x.data)[i]);
-}
-
-// The row that an index names, or `rows` for none. (Apart from the load: a
-// thread loads all its indices before the first of these, whose atomic would
-// hold the later loads back.)
-__device__ __forceinline__ uint32_t row_of(const Index& x, int64_t t) {
-  if (t >= 0 && t < x.rows && !(x.has_padding && t == x.padding)) return uint32_t(t);
-  if (!(x.has_padding && t == x.padding)) atomicOr(&g_token_fault, kFaultTokenRange);
-  return uint32_t(x.rows);
-}
 
 // The tokens at `at(j)`, j < I, where that is below n: from the caller's indices
 // in the first pass, else from the pass before.

@@ -140,9 +140,12 @@ def _workspace_bytes(count, rows, width, consume, ordered):
 
 
 def _workspace(count, rows, width, consume, ordered, like):
-    """A call's workspace as a tensor: (tensor, bytes)."""
+    """A call's workspace: (tensor or None, address or None, bytes)."""
     need = _workspace_bytes(count, rows, width, consume, ordered)
-    return like.new_empty(need, dtype=torch.uint8), need
+    if need == 0:
+        return None, None, 0
+    workspace = like.new_empty(need, dtype=torch.uint8)
+    return workspace, workspace.data_ptr(), need
 
 
 def _lookup(table, index, scale, padding_index, p, seed, offset):
@@ -175,10 +178,10 @@ def lookup_gradient(grad, index, rows, *, scale=1.0, padding_index=None, p=0.0, 
     tokens, alive = _tokens(index, rows, padding_index, order, count, device)
     out = grad.new_empty((rows, width))
     if out.numel():
-        workspace, need = _workspace(count, rows, width, 0, order is not None, out)
+        space = _workspace(count, rows, width, 0, order is not None, out)
         launch(device, "embedding gradient", native.library().clad3dgs_embedding_gradient, kind,
                count, rows, width, grad.data_ptr(), stride, *tokens, scale, p, seed, number,
-               address, out.data_ptr(), workspace.data_ptr(), need)
+               address, out.data_ptr(), space[1], space[2])
     return out
 
 
@@ -216,11 +219,11 @@ def consume_torch_adam(table, first, second, grad, index, *, rate, bias1, bias2_
         a < d and c < b for k, (a, b) in enumerate(spans) for c, d in spans[k + 1:] + read),
         "table, moments, gradient and indices must be disjoint")
     if size:
-        workspace, need = _workspace(count, rows, width, 1, order is not None, table)
+        space = _workspace(count, rows, width, 1, order is not None, table)
         launch(device, "embedding consume", native.library().clad3dgs_embedding_consume_torch_adam,
                kind, count, rows, width, grad.data_ptr(), stride, *tokens, scale, p, seed, number,
                address, spans[0][0], spans[1][0], spans[2][0], rate,
-               native.TorchAdamConfig(bias1, bias2_sqrt), workspace.data_ptr(), need)
+               native.TorchAdamConfig(bias1, bias2_sqrt), space[1], space[2])
 
 
 class _Lookup(torch.autograd.Function):

@@ -24,7 +24,7 @@ ORDER = dict(n=200_000, rows=4, index=256, index_bits=64, has_padding=0, padding
 LOOKUP = dict(type=0, n=10, rows=4, width=8, table=256, table_stride=8, index=512, index_bits=64,
               has_padding=0, padding=0, scale=1.0, p=0.0, seed=0, offset=0, offset_device=None,
               out=1024, stream=0)
-GRADIENT = dict(type=0, n=10, rows=4, width=8, grad=256, grad_stride=8, index=None, index_bits=0,
+GRADIENT = dict(type=0, n=1000, rows=4, width=8, grad=256, grad_stride=8, index=None, index_bits=0,
                 has_padding=0, padding=0, order=512, scale=1.0, p=0.0, seed=0, offset=0,
                 offset_device=None, out=1024, workspace=2048, workspace_bytes=1 << 20, stream=0)
 NAN, INF = float("nan"), float("inf")
@@ -108,6 +108,9 @@ def test_workspaces():
     assert sizes == sorted(sizes) and sizes[2] > 0  # few tokens need none
     assert (lib.clad3dgs_embedding_workspace(70_000, 5, 5, 0, 0)
             >= lib.clad3dgs_embedding_workspace(70_000, 5, 5, 0, 1) + 8 * 70_000)
-    few, many = (lib.clad3dgs_embedding_workspace(n, 4096, 48, 0, 1) for n in (10, 1_000_000))
+    few, many = (lib.clad3dgs_embedding_workspace(n, 4096, 48, 0, 1) for n in (1000, 1_000_000))
     assert 0 < few < many
-    assert lib.clad3dgs_embedding_workspace(10, 4096, 48, 1, 1) >= few + 4 * 4096 + 10 * 48 * 4
+    assert lib.clad3dgs_embedding_workspace(1000, 4096, 48, 1, 1) >= few + 4 * 4096 + 1000 * 48 * 4
+    # Few tokens and a small table need none; a large table does.
+    assert lib.clad3dgs_embedding_workspace(512, 4096, 48, 1, 0) == 0
+    assert lib.clad3dgs_embedding_workspace(512, 40960, 48, 0, 0) > 0

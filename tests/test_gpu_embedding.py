@@ -240,12 +240,13 @@ def test_infinities_and_nan_stay_where_they_are(cuda):
     assert np.array_equal(torch.isnan(got).cpu().numpy(), kept) and not got.nan_to_num().any()
 
 
-def test_an_order_that_no_sort_made_stays_in_bounds(cuda):
+@pytest.mark.parametrize("n", [300, 5000])
+def test_an_order_that_no_sort_made_stays_in_bounds(cuda, n):
     """A TokenOrder is an ordinary tensor: whatever it holds, nothing outside the
     gradient and the table is touched (what comes out is then anything)."""
     import embedding
 
-    rows, width, n = 40, 48, 5000
+    rows, width = 40, 48
     _, index, grad = _case(n, rows, width, torch.float32, cuda)
     room = torch.full((rows + 200, width), 7.0, device=cuda)  # the table lies inside
     state = [room[100:100 + rows], *(_adam_state(rows, width, cuda)[1:])]
@@ -638,3 +639,23 @@ def test_odd_rows_through_the_dropout(cuda, dtype, n, rows, width):
     _check_lookup(embedding.lookup(table, index, **how), table, index, 0.7, 0.35, dtype)
     _check_gradient(embedding.lookup_gradient(grad, index, rows, **how), grad, index, rows, 0.7,
                     0.35, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,rows,width", [(1, 1, 1), (2, 3, 4), (63, 9, 48), (64, 200, 45),
+                                          (65, 1, 7), (511, 5461, 48), (512, 2, 130),
+                                          (512, 5461, 48), (513, 5461, 48), (512, 5462, 48),
+                                          (3, 1, 262_144), (3, 1, 262_145)])
+@pytest.mark.parametrize("p", [0.0, 0.4])
+def test_around_the_border_of_few_tokens(cuda, dtype, n, rows, width, p):
+    """Both sides of 512 tokens and of 2^18 elements; a given order gives the same
+    bits as the call's own."""
+    import embedding
+
+    for kind, padding in (("same", False), ("skewed", True), ("distinct", False)):
+        _, index, grad = _case(n, rows, width, dtype, cuda, kind=kind, bits=32, padding=padding)
+        how = dict(scale=-0.6, p=p, seed=SEED, offset=OFFSET)
+        got = embedding.lookup_gradient(grad, index, rows, padding_index=-1, **how)
+        _check_gradient(got, grad, index, rows, -0.6, p, dtype)
+        order = embedding.token_order(index, rows, padding_index=-1)
+        assert torch.equal(got, embedding.lookup_gradient(grad, None, rows, order=order, **how))
