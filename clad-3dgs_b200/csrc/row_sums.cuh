@@ -552,12 +552,19 @@ __global__ void __launch_bounds__(kThreads)
 // comparing each with all, then eight lanes share the tokens of a vector of the
 // table and add up in a fixed tree. A call on 37 tokens and 1000 x 45 f32 takes
 // 11 us instead of 17, Adam of 60 x 48 with 184 tokens 13 instead of 22.
-constexpr int kFewTokens = 512;
-constexpr int64_t kSmallTable = int64_t(1) << 18;  // elements
+//
+// The GPU's time must stay below the host's as well: at 128 tokens 5 us for 1365
+// x 48 and 7 for 64 x 1024 (10 and 10 in two launches), at 256 tokens 5 to 8 us for
+// 50 x 48 (7 to 8) but 12 for 1365 x 48 (11) and 14 for 64 x 1024 (11), at 512 tokens
+// 17 for a single row of 16 (10).
+constexpr int kFewTokens = 256;
+constexpr int kFewThreads = 256;
+constexpr int64_t kSmallTable = int64_t(1) << 16;  // elements
+constexpr int64_t kSmallWork = int64_t(1) << 23;   // tokens x elements
 constexpr int kSharing = 8;
 
 inline bool few(int64_t n, int64_t rows, int64_t width) {
-  return n > 0 && n <= kFewTokens && rows * width <= kSmallTable;
+  return n > 0 && n <= kFewTokens && rows * width <= kSmallTable && n * rows * width <= kSmallWork;
 }
 
 // Adam as what becomes of a row's sums.
@@ -586,7 +593,7 @@ struct Update {
 // total: vectors of the table. The tokens come from a.order if it is given, else
 // from index.
 template <class T, int V, bool kDrop, class End>
-__global__ void __launch_bounds__(kFewTokens)
+__global__ void __launch_bounds__(kFewThreads)
     few_kernel(const __grid_constant__ Args<T> a, const tokens::Index index, uint32_t total,
                const Narrow vectors, const End end) {
   wait_before();
@@ -601,7 +608,7 @@ __global__ void __launch_bounds__(kFewTokens)
     }
   } else {
     const uint32_t key = me < n ? tokens::row_of(index, tokens::raw_index(index, me)) : kNoRow;
-    keys[me] = key;
+    if (me < n) keys[me] = key;
     __syncthreads();
     if (me < n) {
       int rank = 0;
@@ -621,7 +628,7 @@ __global__ void __launch_bounds__(kFewTokens)
     return low;
   };
   const int share = me % kSharing;
-  constexpr uint32_t kVectors = kFewTokens / kSharing;  // of a block at once
+  constexpr uint32_t kVectors = kFewThreads / kSharing;  // of a block at once
   for (uint32_t first = blockIdx.x * kVectors; first < total; first += gridDim.x * kVectors) {
     const uint32_t at = first + me / kSharing;
     const uint32_t row = vectors.quotient(at);
@@ -655,9 +662,9 @@ template <class T, int V, class End>
 cudaError_t run_few_vectors(const Args<T>& a, const tokens::Index& index, const End& end,
                             bool drop, cudaStream_t stream) {
   const int64_t vectors = a.width / V, total = a.rows * vectors;
-  const int64_t blocks = (total + kFewTokens / kSharing - 1) / (kFewTokens / kSharing);
+  const int64_t blocks = (total + kFewThreads / kSharing - 1) / (kFewThreads / kSharing);
   auto* kernel = drop ? few_kernel<T, V, true, End> : few_kernel<T, V, false, End>;
-  return launch_after(kernel, unsigned(std::min<int64_t>(blocks, kSms * 3)), kFewTokens, 0, stream,
+  return launch_after(kernel, unsigned(std::min<int64_t>(blocks, kSms * 6)), kFewThreads, 0, stream,
                       a, index, uint32_t(total), Narrow(vectors), end);
 }
 

@@ -112,5 +112,6 @@ def test_workspaces():
     assert 0 < few < many
     assert lib.clad3dgs_embedding_workspace(1000, 4096, 48, 1, 1) >= few + 4 * 4096 + 1000 * 48 * 4
     # Few tokens and a small table need none; a large table does.
-    assert lib.clad3dgs_embedding_workspace(512, 4096, 48, 1, 0) == 0
-    assert lib.clad3dgs_embedding_workspace(512, 40960, 48, 0, 0) > 0
+    sizes = [lib.clad3dgs_embedding_workspace(n, rows, 48, 1, 0) > 0
+             for n, rows in ((128, 1365), (128, 1366), (256, 682), (256, 683), (257, 1))]
+    assert sizes == [False, True, False, True, True]
