@@ -278,7 +278,8 @@ struct Tokens {
   // The arguments of the sums; sorts first where it has to.
   template <class T>
   cudaError_t prepare(sums::Args<T>* a, const void* grad, int64_t stride,
-                      const CounterMask& mask, float factor, cudaStream_t stream) const {
+                      const CounterMask& mask, float factor, const tokens::Fill& fill,
+                      cudaStream_t stream) const {
     a->n = n;
     a->rows = rows;
     a->width = width;
@@ -292,7 +293,7 @@ struct Tokens {
     uint2* sorted = reinterpret_cast<uint2*>(workspace);
     a->order = sorted;
     return tokens::sort_tokens(n, index, sorted, workspace + round_up(size_t(n) * sizeof(uint2)),
-                               stream);
+                               fill, stream);
   }
 };
 
@@ -321,7 +322,7 @@ extern "C" int clad3dgs_token_order(int64_t n, int64_t rows, const void* index, 
   if (workspace_bytes < need) return refuse(what, "workspace too small");
   const tokens::Index x{index, index_bits == 64, has_padding != 0, padding, rows};
   return status(what, tokens::sort_tokens(n, x, reinterpret_cast<uint2*>(order), workspace,
-                                          stream));
+                                          tokens::Fill{}, stream));
 }
 
 extern "C" int clad3dgs_embedding_lookup(int type, int64_t n, int64_t rows, int64_t width,
@@ -374,7 +375,7 @@ extern "C" int clad3dgs_embedding_gradient(int type, int64_t n, int64_t rows, in
     using T = decltype(zero);
     sums::Args<T> a{};
     const cudaError_t e =
-        tokens.prepare(&a, grad, grad_stride, mask, factor_of(scale, p), stream);
+        tokens.prepare(&a, grad, grad_stride, mask, factor_of(scale, p), tokens::Fill{}, stream);
     return e == cudaSuccess ? sums::gradient(a, tokens.index, static_cast<T*>(out), p > 0.0, stream) : e;
   };
   return status(what, type == CLAD3DGS_F32   ? go(float())
@@ -406,10 +407,18 @@ extern "C" int clad3dgs_embedding_consume_torch_adam(
     using T = decltype(zero);
     sums::Args<T> a{};
     cudaError_t e = cudaSuccess;
-    if (n > 0 && !sums::few(n, rows, width))
-      e = sums::Kept(tokens.partial(), n, rows, width).clear(rows, stream);
+    tokens::Fill fill;
+    if (n > 0 && !sums::few(n, rows, width)) {
+      // The slots of few rows are cleared by the sort, if there is one.
+      const sums::Kept kept(tokens.partial(), n, rows, width);
+      if (tokens.sorts() && rows <= (1 << 18))
+        fill = {reinterpret_cast<uint4*>(kept.slots),
+                int64_t(sums::slot_bytes(rows) / sizeof(uint4))};
+      else
+        e = kept.clear(rows, stream);
+    }
     if (e == cudaSuccess)
-      e = tokens.prepare(&a, grad, grad_stride, mask, factor_of(scale, p), stream);
+      e = tokens.prepare(&a, grad, grad_stride, mask, factor_of(scale, p), fill, stream);
     return e == cudaSuccess ? sums::consume(a, tokens.index, adam, p > 0.0, stream) : e;
   };
   return status(what, type == CLAD3DGS_F32   ? go(float())
