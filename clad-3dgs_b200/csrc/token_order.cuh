@@ -123,14 +123,20 @@ struct Fill {
   }
 };
 
+// Digits have nine bits at most: with 10 or 11 a pass less is needed for some
+// tables, but costs more than it saves (1.1M tokens over 2000 rows 31 us in two
+// passes, 41 in one; over a million rows 50 in three, 55 in two).
+constexpr int kDigitBits = 9;
 constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
 
 // ---- one cluster ----
 
-constexpr int kClusterBits = 9;
 constexpr int kMostBlocks = 8;  // of a cluster
-constexpr int kSmall = kMostBlocks * kSortThreads * 8;
+// Up to here the cluster is as fast as many blocks or faster (32000 tokens over
+// 4096 rows 13.6 against 15.6 us, 65000 tokens 21.4 against 16.1) and takes
+// fewer launches.
+constexpr int kSmall = kMostBlocks * kSortThreads * 4;
 
 // Block r of the cluster holds the tokens [r * tile, (r + 1) * tile) of the list
 // as sorted so far, tile = I * kSortThreads.
@@ -210,7 +216,7 @@ template <int I>
 cudaError_t cluster_sort(int64_t n, const Index& index, uint2* order, const Fill& fill,
                          cudaStream_t stream) {
   const int all = key_bits(index.rows);
-  const int passes = (all + kClusterBits - 1) / kClusterBits, bits = (all + passes - 1) / passes;
+  const int passes = (all + kDigitBits - 1) / kDigitBits, bits = (all + passes - 1) / passes;
   unsigned blocks = 1;
   while (int64_t(blocks) * I * kSortThreads < n) blocks *= 2;
   const size_t shared = size_t(I) * kSortThreads * sizeof(uint2) +
@@ -237,7 +243,6 @@ cudaError_t cluster_sort(int64_t n, const Index& index, uint2* order, const Fill
 
 // ---- many blocks ----
 
-constexpr int kSortBits = 11;
 constexpr int kSortBlocks = 148;
 
 struct SortPlan {
@@ -253,10 +258,13 @@ inline SortPlan sort_plan(int64_t n, int64_t rows) {
   SortPlan p{};
   if (n <= kSmall) return p;
   const int all = key_bits(rows);
-  p.passes = (all + kSortBits - 1) / kSortBits;
+  p.passes = (all + kDigitBits - 1) / kDigitBits;
   p.bits = (all + p.passes - 1) / p.passes;
-  // Small tiles while they leave no block more than one.
-  p.items = n <= int64_t(kSortBlocks) * kSortThreads * 2 ? 2 : 8;
+  // The smallest tiles that leave no block more than one (250000 tokens over 4096
+  // rows: 20, 21 and 29 us with two, four and eight tokens a thread; 500000: 27, 26
+  // and 31; 1.1M: 40, 36 and 33).
+  const int64_t threads = int64_t(kSortBlocks) * kSortThreads;
+  p.items = n <= threads * 2 ? 2 : n <= threads * 4 ? 4 : 8;
   const int64_t tiles = (n + kSortThreads * p.items - 1) / (kSortThreads * p.items);
   p.tiles = int((tiles + kSortBlocks - 1) / kSortBlocks);
   p.blocks = int((tiles + p.tiles - 1) / p.tiles);
@@ -273,7 +281,7 @@ __global__ void __launch_bounds__(kSortThreads)
                  int bits, uint32_t* __restrict__ counts, const Fill fill) {
   wait_before();
   fill.run();
-  __shared__ uint32_t bins[1 << kSortBits];
+  __shared__ uint32_t bins[1 << kDigitBits];
   const int digits = 1 << bits;
   for (int d = threadIdx.x; d < digits; d += kSortThreads) bins[d] = 0;
   __syncthreads();
@@ -401,13 +409,15 @@ cudaError_t large_sort(int64_t n, const Index& index, const SortPlan& p, uint2* 
 inline cudaError_t sort_tokens(int64_t n, const Index& index, uint2* order, void* workspace,
                                const Fill& fill, cudaStream_t stream) {
   // As many blocks as give each thread one token, then more tokens a thread.
-  if (n <= kSmall / 8) return cluster_sort<1>(n, index, order, fill, stream);
-  if (n <= kSmall / 4) return cluster_sort<2>(n, index, order, fill, stream);
-  if (n <= kSmall / 2) return cluster_sort<4>(n, index, order, fill, stream);
-  if (n <= kSmall) return cluster_sort<8>(n, index, order, fill, stream);
+  if (n <= kSmall / 4) return cluster_sort<1>(n, index, order, fill, stream);
+  if (n <= kSmall / 2) return cluster_sort<2>(n, index, order, fill, stream);
+  if (n <= kSmall) return cluster_sort<4>(n, index, order, fill, stream);
   const SortPlan p = sort_plan(n, index.rows);
-  return p.items == 2 ? large_sort<2>(n, index, p, order, workspace, fill, stream)
-                      : large_sort<8>(n, index, p, order, workspace, fill, stream);
+  switch (p.items) {
+    case 2: return large_sort<2>(n, index, p, order, workspace, fill, stream);
+    case 4: return large_sort<4>(n, index, p, order, workspace, fill, stream);
+    default: return large_sort<8>(n, index, p, order, workspace, fill, stream);
+  }
 }
 
 }  // namespace tokens

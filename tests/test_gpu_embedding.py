@@ -114,7 +114,9 @@ def test_gradient(cuda, dtype, n, rows, width, p):
 
 @pytest.mark.parametrize("kind", ["uniform", "skewed", "same", "sorted", "distinct"])
 @pytest.mark.parametrize("n,rows", [(1, 1), (100, 1000), (4096, 255), (4097, 256), (8191, 1023),
-                                    (8193, 1024), (50_000, 70_000), (16_385, 70_000), (65_537, 31), (300_001, 4096), (310_000, 2047),
+                                    (8193, 1024), (50_000, 70_000), (16_385, 70_000), (32_768, 5), (32_769, 600),
+                                    (65_537, 31), (303_104, 4096), (303_105, 2047),
+                                    (606_209, 511),
                                     (65_537, 3_000_000)])
 def test_order(cuda, kind, n, rows):
     """The stable order, tokens without a row last."""
