@@ -203,8 +203,53 @@ __device__ __forceinline__ Vec<T, V> read_once(const T* from) {
   return v;
 }
 
+// Which of the rows first to first + 31 the order names (bits). The warp looks
+// up where the 32 rows begin and end with 32 probes a step, both at once (four
+// steps for a million tokens, where a lane alone takes twenty), and then reads
+// what lies between.
+__device__ inline unsigned named_rows(int64_t n, const uint2* order, int64_t first) {
+  const int lane = threadIdx.x & 31;
+  int64_t low[2] = {0, 0}, high[2] = {n, n};
+  while (high[0] > low[0] || high[1] > low[1]) {
+    int64_t probe[2];
+    uint32_t key[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int64_t length = high[e] - low[e];
+      probe[e] = length > 32 ? low[e] + length * (lane + 1) / 33 : low[e] + lane;
+      key[e] = probe[e] < high[e] ? order[probe[e]].x : kNoRow;
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int less = __popc(__ballot_sync(~0u, key[e] < first + 32 * e));
+      const int64_t last = __shfl_sync(~0u, probe[e], less > 0 ? less - 1 : 0);
+      const int64_t next = __shfl_sync(~0u, probe[e], less < 32 ? less : 31);
+      if (high[e] - low[e] > 32) {
+        if (less < 32) high[e] = next;
+        if (less > 0) low[e] = last + 1;
+      } else {
+        low[e] = high[e] = low[e] + less;
+      }
+    }
+  }
+  unsigned named = 0;
+  if (low[1] - low[0] <= 1024) {
+    for (int64_t i = low[0] + lane; i < low[1]; i += 32)
+      named |= 1u << (unsigned(order[i].x - first) & 31);
+  } else {
+    int64_t from = low[0], to = low[1];
+    while (from < to) {
+      const int64_t middle = (from + to) / 2;
+      if (order[middle].x < first + lane) from = middle + 1;
+      else to = middle;
+    }
+    if (from < low[1] && order[from].x == first + lane) named = 1u << lane;
+  }
+  return __reduce_or_sync(~0u, named);
+}
+
 // Rows that no token names: a gradient of zero. One warp takes 32 rows and one
-// slice of columns; each lane looks one of the rows up in the order.
+// slice of columns.
 template <int V, class End>
 __device__ void write_rest(int64_t n, int64_t rows, int64_t width, const uint2* order,
                            const End& end) {
@@ -213,21 +258,21 @@ __device__ void write_rest(int64_t n, int64_t rows, int64_t width, const uint2* 
   const int64_t first = job / slices * 32;
   if (first >= rows) return;
   const int lane = threadIdx.x & 31;
-  const int64_t mine = first + lane;
-  bool named = true;
-  if (mine < rows) {
-    int64_t low = 0, high = n;
-    while (low < high) {
-      const int64_t middle = (low + high) / 2;
-      if (order[middle].x < mine) low = middle + 1;
-      else high = middle;
-    }
-    named = low < n && order[low].x == mine;
+  unsigned left = ~named_rows(n, order, first);
+  if (rows - first < 32) left &= (1u << (rows - first)) - 1;
+  const float zero[V] = {};
+  const int64_t vectors = width / V;
+  if (vectors <= 16) {  // several rows at once
+    int lanes = 1;
+    while (lanes < vectors) lanes *= 2;
+    const int column = lane % lanes;
+    for (int r = lane / lanes; r < 32; r += 32 / lanes)
+      if ((left >> r & 1) && column < vectors)
+        end.template put<V>((first + r) * width + column * V, zero);
+    return;
   }
-  unsigned left = __ballot_sync(~0u, !named);
   const int64_t column = (job % slices * 32 + lane) * V;
   if (column >= width) return;
-  const float zero[V] = {};
   while (left) {
     end.template put<V>((first + __ffs(left) - 1) * width + column, zero);
     left &= left - 1;
