@@ -532,7 +532,8 @@ int clad3dgs_embedding_lookup(int type, int64_t n, int64_t rows, int64_t width,
  * [n][width] with a row stride in elements. The tokens are given by order, from
  * clad3dgs_token_order of the same n and rows, or with order null by index,
  * index_bits and padding (as there), which the call then sorts for itself. Sums
- * are 32-bit floats in an order that depends on the sizes alone. workspace:
+ * are 32-bit floats in an order that depends on the sizes alone (64 bits where
+ * parts of very long rows meet). workspace:
  * clad3dgs_embedding_workspace bytes (consume = 0 here, 1 for the Adam entry
  * below; ordered = whether order is given), 256-byte aligned. */
 size_t clad3dgs_embedding_workspace(int64_t n, int64_t rows, int64_t width, int consume,
