@@ -95,6 +95,11 @@ def test_far_elements_and_large_numbers(cuda):
     for row in (0, 1, 4095, 4096, 4099):
         kept = draws.keep(row * width + np.arange(1000), 0.5, 2 ** 63 + 11, 2 ** 64 - 1)
         assert np.array_equal(y[row, :1000].cpu().numpy() > 0, kept), row
+    # The packed result once more, in place under another offset.
+    before = y[4099, :1000].clone()
+    dropout.apply(y, 0.5, 5, 6, out=y)
+    kept = draws.keep(4099 * width + np.arange(1000), 0.5, 5, 6)
+    assert np.array_equal(y[4099, :1000].cpu().numpy(), before.cpu().numpy() * kept * 2)
 
 
 @pytest.mark.parametrize("dtype", TYPES)

@@ -280,6 +280,27 @@ def test_far_rows(cuda):
     assert [int(got[r].any()) for r in (1, 65_535, 65_537, rows - 2)] == [0] * 4
 
 
+def test_far_tokens(cuda):
+    """Output elements past 2^32, aligned and odd rows: the lookup's zeros are the
+    generator's, and the gradient counts what the lookup kept."""
+    import embedding
+
+    n = 66_000
+    for width in (65_600, 65_601):
+        table = torch.ones(2, width, dtype=torch.float16, device=cuda)
+        index = torch.arange(n, device=cuda) % 2
+        y = embedding.lookup(table, index, p=0.5, seed=SEED, offset=OFFSET)
+        for token in (0, 65_500, n - 1):
+            kept = draws.keep(token * width + np.arange(500), 0.5, SEED, OFFSET)
+            assert np.array_equal(y[token, :500].cpu().numpy() > 0, kept)
+        columns = [0, 1, 30_000, width - 1]
+        want = torch.stack([(y[r::2][:, columns] > 0).sum(0) for r in (0, 1)])
+        del y
+        grad = torch.ones(1, width, device=cuda).expand(n, width)
+        got = embedding.lookup_gradient(grad, index, 2, scale=0.5, p=0.5, seed=SEED, offset=OFFSET)
+        assert torch.equal(got[:, columns], want.float())
+
+
 # ---------------------------------------------------------------------------
 # Adam.
 
