@@ -85,15 +85,17 @@ __global__ void __launch_bounds__(kThreads)
     raw[u] = at < total ? tokens::raw_index(index, i) : 0;
   }
   Vec<T, V> v[U];
+  bool bad = false;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     v[u] = {};
     if (first + u * kThreads < total) {
-      const uint32_t row = tokens::row_of(index, raw[u]);
+      const uint32_t row = tokens::row_of(index, raw[u], &bad);
       if (row < index.rows)
         v[u] = *reinterpret_cast<const Vec<T, V>*>(table + row * table_stride + column[u]);
     }
   }
+  tokens::report(bad);
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const Number at = first + u * kThreads;
@@ -123,14 +125,15 @@ __global__ void __launch_bounds__(kThreads)
   if (at >= total) return;
   Number i = width.quotient(at), column = at - i * width.divisor;
   Vec<T, V> v{};
-  uint32_t row = tokens::row_of(index, tokens::raw_index(index, i));
+  bool bad = false;
+  uint32_t row = tokens::row_of(index, tokens::raw_index(index, i), &bad);
   if constexpr (kShort) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       if (at + j < total) {
         if (column == width.divisor) {
           column = 0;
-          row = tokens::row_of(index, tokens::raw_index(index, ++i));
+          row = tokens::row_of(index, tokens::raw_index(index, ++i), &bad);
         }
         if (row < index.rows) v.v[j] = table[row * table_stride + column];
         ++column;
@@ -141,7 +144,7 @@ __global__ void __launch_bounds__(kThreads)
     const int border = width.divisor - column < V ? int(width.divisor - column) : V;
     const int count = total - at < V ? int(total - at) : V;
     uint32_t next = uint32_t(index.rows);
-    if (border < count) next = tokens::row_of(index, tokens::raw_index(index, i + 1));
+    if (border < count) next = tokens::row_of(index, tokens::raw_index(index, i + 1), &bad);
     const T* here = table + row * table_stride + column;
     const T* there = table + next * table_stride - border;
     const int until = row < index.rows ? (border < count ? border : count) : 0;
@@ -152,6 +155,7 @@ __global__ void __launch_bounds__(kThreads)
       else if (j >= from && j < count) v.v[j] = there[j];
     }
   }
+  tokens::report(bad);
   bool keep[V];
   if (kDrop) mask_vector<V, Number>(mask, offset, uint64_t(at), keep);
   v = finish<T, V, kDrop>(v, keep, factor);

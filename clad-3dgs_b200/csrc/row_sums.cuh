@@ -672,7 +672,10 @@ __global__ void __launch_bounds__(kFewThreads)
       sorted[me] = one;
     }
   } else {
-    const uint32_t key = me < n ? tokens::row_of(index, tokens::raw_index(index, me)) : kNoRow;
+    bool bad = false;
+    const uint32_t key =
+        me < n ? tokens::row_of(index, tokens::raw_index(index, me), &bad) : kNoRow;
+    tokens::report(bad);
     if (me < n) keys[me] = key;
     __syncthreads();
     if (me < n) {

@@ -26,13 +26,19 @@ __device__ __forceinline__ int64_t raw_index(const Index& x, int64_t i) {
                 : int64_t(static_cast<const int32_t*>(x.data)[i]);
 }
 
-// The row that an index names, or `rows` for none. (Apart from the load: a
-// thread loads all its indices before the first of these, whose atomic would
-// hold the later loads back.)
-__device__ __forceinline__ uint32_t row_of(const Index& x, int64_t t) {
-  if (t >= 0 && t < x.rows && !(x.has_padding && t == x.padding)) return uint32_t(t);
-  if (!(x.has_padding && t == x.padding)) atomicOr(&g_token_fault, kFaultTokenRange);
-  return uint32_t(x.rows);
+// The row that an index names, or `rows` for none; *bad is set for an index
+// outside the table that is not the padding.
+__device__ __forceinline__ uint32_t row_of(const Index& x, int64_t t, bool* bad) {
+  const bool inside = uint64_t(t) < uint64_t(x.rows);
+  const bool padding = x.has_padding && t == x.padding;
+  *bad |= !inside && !padding;
+  return uint32_t(inside && !padding ? t : x.rows);
+}
+
+// Once a thread, for all its indices: an atomic between two of them would hold
+// back the loads behind it.
+__device__ __forceinline__ void report(bool bad) {
+  if (bad) atomicOr(&g_token_fault, kFaultTokenRange);
 }
 
 // Adds this file's fault word to *word, and clears it if asked to.

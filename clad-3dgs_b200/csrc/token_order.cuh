@@ -44,9 +44,11 @@ __device__ __forceinline__ void load_pairs(const Index& index, const uint2* from
   int64_t raw[I];
 #pragma unroll
   for (int j = 0; j < I; ++j) raw[j] = at(j) < n ? raw_index(index, at(j)) : 0;
+  bool bad = false;
 #pragma unroll
   for (int j = 0; j < I; ++j)
-    if (at(j) < n) pair[j] = make_uint2(row_of(index, raw[j]), uint32_t(at(j)));
+    if (at(j) < n) pair[j] = make_uint2(row_of(index, raw[j], &bad), uint32_t(at(j)));
+  report(bad);
 }
 
 // Ranks of a tile: thread t of warp w holds the tokens w * 32 * I + 32 * j + lane,
