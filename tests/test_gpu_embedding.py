@@ -683,3 +683,58 @@ def test_around_the_border_of_few_tokens(cuda, dtype, n, rows, width, p):
         _check_gradient(got, grad, index, rows, -0.6, p, dtype)
         order = embedding.token_order(index, rows, padding_index=-1)
         assert torch.equal(got, embedding.lookup_gradient(grad, None, rows, order=order, **how))
+
+
+def test_forked_streams_under_a_graph(cuda):
+    """A capture that forks to a second stream and joins right before a call: the
+    call's kernels then wait for two predecessors."""
+    import dropout
+    import embedding
+
+    n, rows, width = 5000, 300, 48
+    table, index, grad = _case(n, rows, width, torch.float32, cuda, kind="skewed")
+    state = _adam_state(rows, width, cuda)
+
+    def work(side):
+        main = torch.cuda.current_stream()
+        order = embedding.token_order(index, rows)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            d = dropout.apply(grad, 0.4, 1, 2)
+        a = embedding.lookup(table, index)
+        main.wait_stream(side)
+        g = embedding.lookup_gradient(d, None, rows, order=order)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            b = dropout.apply(a, 0.2, 3, 4)
+        h = embedding.lookup_gradient(a, index, rows)
+        main.wait_stream(side)
+        embedding.consume_torch_adam(*state, b, None, order=order, rate=0.01, bias1=0.5,
+                                     bias2_sqrt=0.5)
+        return g, h, b
+
+    side = torch.cuda.Stream()
+    other = torch.cuda.Stream()
+    with torch.cuda.stream(other):
+        work(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = work(side)
+    for seed in (1, 2):
+        t, i, g = _case(n, rows, width, torch.float32, cuda, kind="skewed", seed=seed)
+        table.copy_(t)
+        index.copy_(i)
+        grad.copy_(g)
+        before = [x.clone() for x in state]
+        graph.replay()
+        torch.cuda.synchronize()
+        after = [x.clone() for x in state]
+        d = dropout.apply(grad, 0.4, 1, 2)
+        a = embedding.lookup(table, index)
+        b = dropout.apply(a, 0.2, 3, 4)
+        assert torch.equal(got[0], embedding.lookup_gradient(d, index, rows))
+        assert torch.equal(got[1], embedding.lookup_gradient(a, index, rows))
+        assert torch.equal(got[2], b)
+        embedding.consume_torch_adam(*before, b, index, rate=0.01, bias1=0.5, bias2_sqrt=0.5)
+        assert all(torch.equal(x, y) for x, y in zip(before, after))
