@@ -64,8 +64,8 @@ __device__ __forceinline__ Vec<T, V> finish(const Vec<T, V>& x, const bool (&kee
 // top; small tables stay in L2). Threads take consecutive vectors of 16 bytes of
 // the output, whatever rows they belong to, so that stores are whole lines, U of
 // them each, all asked for before the first is stored. 1.1M rows of 48 floats
-// from 4096: 40 us (5.3 TB/s; groups of lanes a row 50, one vector a thread
-// 147); 16384 of 2048 bf16 from 131072: 23 us (5.8 TB/s).
+// from 4096: 39 us (5.5 TB/s; groups of lanes a row 50, one vector a thread
+// 147); 16384 of 2048 bf16 from 131072: 20 us (6.8 TB/s).
 template <class T, class Division, int V, int U, bool kDrop>
 __global__ void __launch_bounds__(kThreads)
     lookup_kernel(typename Division::Number total, const Division vectors,
@@ -184,14 +184,20 @@ unsigned grid_of(int64_t work, int64_t each) { return unsigned((work + each - 1)
 template <class T, class Division>
 cudaError_t run_lookup(const Lookup& a, bool aligned) {
   using Number = typename Division::Number;
-  constexpr int V = 16 / sizeof(T), U = 4;
+  constexpr int V = 16 / sizeof(T);
   const T* table = static_cast<const T*>(a.table);
   T* out = static_cast<T*>(a.out);
   if (aligned) {
+    // Two vectors a thread where a warp's belong to one row, whose index is
+    // read once (16384 x 2048 bf16: 19.7 us, 22.7 with four), else four, to have
+    // more of the indices on their way (1.1M x 48 f32: 39 us, 46 with two).
     const int64_t vectors = a.width / V, total = a.n * vectors;
-    auto* kernel =
-        a.drop ? lookup_kernel<T, Division, V, U, true> : lookup_kernel<T, Division, V, U, false>;
-    return launch_after(kernel, grid_of(total, U * kThreads), kThreads, 0, a.stream,
+    const bool wide = vectors >= 32;
+    auto* kernel = wide ? (a.drop ? lookup_kernel<T, Division, V, 2, true>
+                                  : lookup_kernel<T, Division, V, 2, false>)
+                        : (a.drop ? lookup_kernel<T, Division, V, 4, true>
+                                  : lookup_kernel<T, Division, V, 4, false>);
+    return launch_after(kernel, grid_of(total, (wide ? 2 : 4) * kThreads), kThreads, 0, a.stream,
         Number(total), Division(vectors), table, a.stride, a.index, a.factor, a.mask, out);
   }
   const int64_t total = a.n * a.width;
