@@ -48,11 +48,15 @@ constexpr int kLeastTokens = 8;    // of a group: keeps the joins few
 constexpr uint32_t kNoRow = ~0u;
 
 // Rows a thread asks for at once (of each it takes `bytes`), and the blocks that
-// an SM's registers hold.
+// an SM's registers hold (200000 rows of 256 floats, 64 bytes a thread and row: 47
+// us with two blocks, 51 with three; 1M of 48 bf16, 32 bytes: 56 with three, 58 with
+// two).
 constexpr int rows_at_once(int bytes, bool loose) {
   return loose ? 2 : bytes <= 8 ? 8 : bytes <= 16 ? 4 : 2;
 }
-constexpr int blocks_per_sm(int elements) { return elements <= 4 ? 4 : 3; }
+constexpr int blocks_per_sm(int elements, int bytes) {
+  return elements <= 4 ? 4 : bytes < 64 ? 3 : 2;
+}
 
 // How [n][width] gradients are cut: C vectors of `lanes` lanes in a group,
 // `slices` groups a row, `tokens` of one group, `block` of one block.
@@ -83,7 +87,7 @@ inline int lanes_of(int64_t vectors, int c, int64_t* padded) {
   return lanes;
 }
 
-inline Cut cut_of(int64_t n, int64_t width, int vec, int c, int64_t rest) {
+inline Cut cut_of(int64_t n, int64_t width, int vec, int c, int sm_blocks, int64_t rest) {
   const int64_t vectors = (width + vec - 1) / vec;
   Cut cut{};
   int64_t padded;
@@ -92,7 +96,7 @@ inline Cut cut_of(int64_t n, int64_t width, int vec, int c, int64_t rest) {
   // Tokens of a group: as many as fill the GPU in whole waves.
   const int groups = kThreads / cut.lanes;
   // (a few blocks in front for the rows without tokens take places of the first).
-  const int64_t places = int64_t(kSms) * blocks_per_sm(c * vec);
+  const int64_t places = int64_t(kSms) * sm_blocks;
   const int64_t resident = std::max<int64_t>(
       1, (places - (rest < places / 2 ? rest : 0)) / cut.slices * groups);
   const int most = std::max(kLeastTokens, kMostTokens / groups);
@@ -294,7 +298,7 @@ enum Head : unsigned char { kNone = 0, kEnded = 1, kOpen = 2 };
 // begin anywhere and end behind the row, moved one by one (for dropout on odd
 // rows: single elements would draw four words for every one they use).
 template <class T, int V, int C, int R, bool kDrop, bool kLoose, class End>
-__global__ void __launch_bounds__(kThreads, blocks_per_sm(C * V))
+__global__ void __launch_bounds__(kThreads, blocks_per_sm(C * V, C * V * sizeof(T)))
     sum_kernel(const __grid_constant__ Args<T> a, const End end) {
   wait_before();
   if constexpr (End::kRest) {
@@ -772,7 +776,7 @@ inline int vectors_of_lane(int64_t n, int64_t width, int vec, bool floats) {
 template <class T, int V, int C, int R, bool kDrop, bool kLoose, class End>
 cudaError_t run_cut(Args<T> a, const End& end, cudaStream_t stream) {
   a.rest = End::kRest ? rest_blocks(a.rows, a.width, R) : 0;
-  a.cut = cut_of(a.n, a.width, V, C, a.rest);
+  a.cut = cut_of(a.n, a.width, V, C, blocks_per_sm(C * V, C * V * sizeof(T)), a.rest);
   const unsigned grid = unsigned(a.rest + a.cut.blocks * a.cut.slices);
   const cudaError_t e = launch_after(sum_kernel<T, V, C, R, kDrop, kLoose, End>, grid, kThreads, 0,
                                      stream, a, end);
