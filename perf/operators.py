@@ -39,36 +39,36 @@ def _dropout(name, tokens, width, dtype, **more):
 def listed():
     return [
         # One token of a language-sized table: the latency of the smallest call.
-        _lookup("lookup: one token", 1, 65536, 2048, "bf16", "i64", scale=math.sqrt(2048.0)),
+        _lookup("lookup, one token", 1, 65536, 2048, "bf16", "i64", scale=math.sqrt(2048.0)),
         # 1.1M Gaussians taking their 48 SH coefficients from a codebook.
-        _lookup("lookup: codebook colours", 1_100_000, 4096, 48, "f32", "i32"),
+        _lookup("lookup, codebook colours", 1_100_000, 4096, 48, "f32", "i32"),
         # A batch of token embeddings, scaled by the root of the width.
-        _lookup("lookup: token batch", 16384, 131072, 2048, "bf16", "i64",
+        _lookup("lookup, token batch", 16384, 131072, 2048, "bf16", "i64",
                 scale=math.sqrt(2048.0)),
         # Odd sizes, padded tokens and dropout in the same pass.
-        _lookup("lookup: odd with dropout", 100_003, 5003, 77, "f16", "i64", p=0.1,
+        _lookup("lookup, odd with dropout", 100_003, 5003, 77, "f16", "i64", p=0.1,
                 padding=True, scale=0.5),
         # The codebook's gradient: few rows, long sums, a few rows far more used than the rest.
-        {**_lookup("gradient: codebook colours", 1_100_000, 4096, 48, "f32", "i32"),
+        {**_lookup("gradient, codebook colours", 1_100_000, 4096, 48, "f32", "i32"),
          "op": "gradient"},
         # A large table of which a batch names a small part; the rest is zeros.
-        {**_lookup("gradient: token batch", 16384, 131072, 2048, "bf16", "i64",
+        {**_lookup("gradient, token batch", 16384, 131072, 2048, "bf16", "i64",
                    scale=math.sqrt(2048.0)), "op": "gradient"},
         # A small odd one: latency.
-        {**_lookup("gradient: small", 37, 1000, 45, "f32", "i64", p=0.25, padding=True),
+        {**_lookup("gradient, small", 37, 1000, 45, "f32", "i64", p=0.25, padding=True),
          "op": "gradient"},
         # The codebook's training step; assignments stay the same over the steps.
-        {**_lookup("adam: codebook colours", 1_100_000, 8192, 48, "f32", "i32"),
+        {**_lookup("adam, codebook colours", 1_100_000, 8192, 48, "f32", "i32"),
          "op": "adam", "kept": True},
         # A token table's training step, bf16 gradients through the dropout.
-        {**_lookup("adam: token batch", 8192, 32768, 1024, "bf16", "i64", p=0.1, scale=32.0),
+        {**_lookup("adam, token batch", 8192, 32768, 1024, "bf16", "i64", p=0.1, scale=32.0),
          "op": "adam", "kept": False},
         # The opacities of 6M Gaussians.
-        _dropout("dropout: opacities", 6_000_000, 1, "f32"),
+        _dropout("dropout, opacities", 6_000_000, 1, "f32"),
         # Hidden states, forward and backward.
-        _dropout("dropout: states", 16384, 4096, "bf16", backward=True),
+        _dropout("dropout, states", 16384, 4096, "bf16", backward=True),
         # Whole rows dropped, few and odd.
-        _dropout("dropout: rows", 257, 33, "f16", rows_form=True, backward=True, p=0.5),
+        _dropout("dropout, rows", 257, 33, "f16", rows_form=True, backward=True, p=0.5),
     ]
 
 
