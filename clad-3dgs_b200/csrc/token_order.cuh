@@ -132,6 +132,19 @@ constexpr int kDigitBits = 9;
 constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
 
+// Shared memory of the counts by digit (two sums, and one count a warp).
+constexpr size_t digit_bytes(int bits) {
+  return (size_t(1) << bits) * (kSortWarps * sizeof(uint16_t) + 2 * sizeof(uint32_t));
+}
+
+// Lets a kernel have the most that any launch of it asks for. The limit belongs
+// to the kernel, not to a launch: one that followed the launch's own digits
+// would lower it between another host thread's setting and launch.
+template <class Kernel>
+cudaError_t allow_shared(Kernel* kernel, size_t most) {
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(most));
+}
+
 // ---- one cluster ----
 
 constexpr int kMostBlocks = 8;  // of a cluster
@@ -221,10 +234,9 @@ cudaError_t cluster_sort(int64_t n, const Index& index, uint2* order, const Fill
   const int passes = (all + kDigitBits - 1) / kDigitBits, bits = (all + passes - 1) / passes;
   unsigned blocks = 1;
   while (int64_t(blocks) * I * kSortThreads < n) blocks *= 2;
-  const size_t shared = size_t(I) * kSortThreads * sizeof(uint2) +
-                        (size_t(1) << bits) * (kSortWarps * sizeof(uint16_t) + 2 * sizeof(uint32_t));
-  cudaError_t e = cudaFuncSetAttribute(cluster_sort_kernel<I>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared));
+  constexpr size_t kTileBytes = size_t(I) * kSortThreads * sizeof(uint2);
+  const size_t shared = kTileBytes + digit_bytes(bits);
+  cudaError_t e = allow_shared(cluster_sort_kernel<I>, kTileBytes + digit_bytes(kDigitBits));
   if (e != cudaSuccess) return e;
   cudaLaunchAttribute attributes[2]{};
   attributes[0].id = cudaLaunchAttributeClusterDimension;
@@ -385,10 +397,8 @@ cudaError_t large_sort(int64_t n, const Index& index, const SortPlan& p, uint2* 
   uint2* spare = static_cast<uint2*>(workspace);
   uint32_t* counts =
       reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + p.pair_bytes);
-  const size_t shared =
-      (size_t(1) << p.bits) * (2 * sizeof(uint32_t) + kSortWarps * sizeof(uint16_t));
-  cudaError_t e = cudaFuncSetAttribute(
-      scatter_kernel<I>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared));
+  const size_t shared = digit_bytes(p.bits);
+  cudaError_t e = allow_shared(scatter_kernel<I>, digit_bytes(kDigitBits));
   if (e != cudaSuccess) return e;
   const uint2* from = nullptr;
   for (int pass = 0; pass < p.passes; ++pass) {

@@ -738,3 +738,71 @@ def test_forked_streams_under_a_graph(cuda):
         assert torch.equal(got[2], b)
         embedding.consume_torch_adam(*before, b, index, rate=0.01, bias1=0.5, bias2_sqrt=0.5)
         assert all(torch.equal(x, y) for x, y in zip(before, after))
+
+
+def test_threads_sort_by_digits_of_different_widths(cuda):
+    """Host threads whose tables need narrow and wide digits of the same sort
+    kernels (16000 tokens: one cluster; 70000: many blocks). Every call of every
+    thread has to succeed, with the bits of a call alone."""
+    import threading
+
+    import embedding
+
+    sizes = [(16_000, 5), (16_000, 131_072), (70_000, 3), (70_000, 131_072)]
+    rounds, width = 120, 8
+    cases = [_case(n, rows, width, torch.float32, cuda, seed=k) for k, (n, rows) in enumerate(sizes)]
+
+    def call(k, which):
+        (_, rows), (_, index, grad) = sizes[k], cases[k]
+        if which == 0:
+            return [embedding.token_order(index, rows).pairs]
+        if which == 1:
+            return [embedding.lookup_gradient(grad, index, rows)]
+        state = [t.clone() for t in states[k]]
+        embedding.consume_torch_adam(*state, grad, index, rate=0.1, bias1=0.5, bias2_sqrt=0.5)
+        return state
+
+    states = [_adam_state(rows, width, cuda, seed=k) for k, (_, rows) in enumerate(sizes)]
+    want = [[call(k, which) for which in range(3)] for k in range(len(sizes))]
+    torch.cuda.synchronize()
+    done, wrong, errors = [0] * len(sizes), [], []
+
+    def work(k):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for i in range(rounds):
+                    got = call(k, i % 3)
+                    torch.cuda.current_stream().synchronize()
+                    if not all(torch.equal(a, b) for a, b in zip(got, want[k][i % 3])):
+                        wrong.append((k, i))
+                    done[k] += 1
+        except Exception as e:  # a thread's exception does not fail a test by itself
+            errors.append((k, done[k], repr(e)))
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(len(sizes))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors and not wrong and done == [rounds] * len(sizes)
+
+
+@pytest.mark.parametrize("n", [16_000, 70_000])
+def test_digits_of_different_widths_in_one_graph(cuda, n):
+    """A graph that holds the same sort kernel with wide and then with narrow
+    digits, instantiated after both."""
+    import embedding
+
+    _, wide, _ = _case(n, 131_072, 1, torch.float32, cuda, seed=1)
+    _, narrow, _ = _case(n, 3, 1, torch.float32, cuda, seed=2)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = [embedding.token_order(wide, 131_072), embedding.token_order(narrow, 3)]
+    for seed in (3, 4):
+        wide.copy_(_case(n, 131_072, 1, torch.float32, cuda, seed=seed)[1])
+        narrow.copy_(_case(n, 3, 1, torch.float32, cuda, seed=seed)[1])
+        graph.replay()
+        for index, order in zip((wide, narrow), got):
+            i = index.cpu().numpy()
+            place = np.argsort(i, kind="stable")
+            assert np.array_equal(order.pairs.cpu().numpy(), np.stack([i[place], place], axis=1))
