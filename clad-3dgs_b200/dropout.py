@@ -22,6 +22,7 @@ raise RuntimeError before anything is written.
 from __future__ import annotations
 
 import torch
+from torch.autograd.forward_ad import make_dual, unpack_dual
 
 import _native as native
 
@@ -127,14 +128,19 @@ class _Dropout(torch.autograd.Function):
         p, seed, offset, rows = ctx.numbers
         if offset is None:
             offset = ctx.saved_tensors[0]
-        elif not torch.is_grad_enabled():
+        elif not torch.is_grad_enabled() and unpack_dual(grad).tangent is None:
             return _run(grad, p, seed, offset, None, rows), None, None, None, None
         return dropout(grad, p, seed, offset, rows=rows), None, None, None, None
 
 
 def dropout(x, p, seed, offset=0, *, rows=False):
     """x with a share p of its elements (rows=True: of its rows) set to zero and
-    the others scaled by 1 / (1 - p); differentiable any number of times."""
+    the others scaled by 1 / (1 - p); differentiable any number of times, in
+    reverse and in forward mode."""
+    primal, tangent = unpack_dual(x)
+    if tangent is not None:  # the map is linear
+        draw = dict(p=p, seed=seed, offset=offset, rows=rows)
+        return make_dual(dropout(primal, **draw), dropout(tangent, **draw))
     if x.requires_grad and torch.is_grad_enabled():
         return _Dropout.apply(x, p, seed, offset, bool(rows))
     number, address = _check(x, p, seed, offset)

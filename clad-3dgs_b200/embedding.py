@@ -6,7 +6,8 @@ token names a row of `table` [rows, width].
 
 * `lookup(table, index, scale=..., p=..., seed=..., offset=...)`: the rows, times
   `scale`, with the dropout of `dropout.dropout(out, p, seed, offset)` in the
-  same pass; differentiable once in the table.
+  same pass; differentiable in the table, once in reverse mode and in forward
+  mode.
 * `lookup_gradient(grad, index, rows, ...)`: the adjoint, a dense [rows, width].
 * `consume_torch_adam(table, first, second, grad, index, ...)`: the adjoint and
   torch-fused Adam on the table in one call, like the SH consume entries; of
@@ -35,6 +36,7 @@ from functools import lru_cache
 from typing import NamedTuple
 
 import torch
+from torch.autograd.forward_ad import make_dual, unpack_dual
 
 import _native as native
 from dropout import TYPES, check_draw, launch
@@ -170,6 +172,12 @@ def lookup_gradient(grad, index, rows, *, scale=1.0, padding_index=None, p=0.0, 
     """The table's gradient [rows, width] (grad's type) of a `lookup` with these
     arguments whose output has the gradient `grad` [*index.shape, width]. With
     `order` (from `token_order`), index and padding_index are not read."""
+    primal, tangent = unpack_dual(grad)
+    if tangent is not None:  # as in lookup
+        how = dict(scale=scale, padding_index=padding_index, p=p, seed=seed, offset=offset,
+                   order=order)
+        return make_dual(lookup_gradient(primal, index, rows, **how),
+                         lookup_gradient(tangent, index, rows, **how))
     grad, kind, count, width, stride = _gradient_matrix(grad)
     device = grad.device
     _check_rows(rows)
@@ -250,6 +258,11 @@ def lookup(table, index, *, scale=1.0, padding_index=None, p=0.0, seed=0, offset
     """scale * table[index], of the table's type, shaped [*index.shape, width]; with
     p > 0 through the dropout of (p, seed, offset). `order` (from `token_order`
     of the same index, rows and padding) spares the backward pass its sort."""
+    primal, tangent = unpack_dual(table)
+    if tangent is not None:  # the map is linear in the table
+        how = dict(scale=scale, padding_index=padding_index, p=p, seed=seed, offset=offset,
+                   order=order)
+        return make_dual(lookup(primal, index, **how), lookup(tangent, index, **how))
     if table.requires_grad and torch.is_grad_enabled():
         if order is not None:
             _tokens(None, table.shape[0], None, order, index.numel(), table.device)

@@ -221,3 +221,28 @@ def test_other_stream(cuda):
         got = dropout.dropout(x, 0.5, 8, 9)
     side.synchronize()
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("offset_on_device", [False, True])
+@pytest.mark.parametrize("rows", [False, True])
+def test_forward_mode_derivatives(cuda, rows, offset_on_device):
+    """The map is linear: a tangent goes through the same draw, in the forward
+    pass and in the gradient's own derivative."""
+    import dropout
+    from torch.autograd import forward_ad
+
+    x, tangent = _input((60, 33), torch.float32, cuda), _input((60, 33), torch.float32, cuda, seed=1)
+    offset = torch.full((1,), 7, device=cuda) if offset_on_device else 7
+    drop = lambda v: dropout.dropout(v, 0.5, 3, offset, rows=rows)
+    want, moved = drop(x), drop(tangent)
+    for grad_needed in (False, True):
+        leaf = x.clone().requires_grad_(grad_needed)
+        with forward_ad.dual_level():
+            y = drop(forward_ad.make_dual(leaf, tangent))
+            value, slope = forward_ad.unpack_dual(y)
+            assert torch.equal(value, want) and torch.equal(slope, moved)
+            if grad_needed:
+                (g,) = torch.autograd.grad((y * y).sum(), leaf)
+                g, dg = forward_ad.unpack_dual(g)
+                assert torch.equal(g, drop(2 * want)) and torch.equal(dg, drop(2 * moved))
+            assert forward_ad.unpack_dual(drop(x)).tangent is None

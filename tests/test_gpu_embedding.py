@@ -806,3 +806,30 @@ def test_digits_of_different_widths_in_one_graph(cuda, n):
             i = index.cpu().numpy()
             place = np.argsort(i, kind="stable")
             assert np.array_equal(order.pairs.cpu().numpy(), np.stack([i[place], place], axis=1))
+
+
+@pytest.mark.parametrize("offset_on_device", [False, True])
+def test_forward_mode_derivatives(cuda, offset_on_device):
+    """The lookup is linear in the table: a tangent goes through the same lookup,
+    in the forward pass and in the gradient's own derivative."""
+    import embedding
+    from torch.autograd import forward_ad
+
+    table, index, _ = _case(300, 40, 48, torch.float32, cuda, kind="skewed")
+    tangent = torch.randn(40, 48, device=cuda, generator=torch.Generator(device=cuda).manual_seed(1))
+    offset = torch.full((1,), OFFSET, device=cuda) if offset_on_device else OFFSET
+    how = dict(scale=0.5, p=0.25, seed=SEED, offset=offset)
+    want, moved = embedding.lookup(table, index, **how), embedding.lookup(tangent, index, **how)
+    for grad_needed in (False, True):
+        leaf = table.clone().requires_grad_(grad_needed)
+        with forward_ad.dual_level():
+            y = embedding.lookup(forward_ad.make_dual(leaf, tangent), index, **how)
+            value, slope = forward_ad.unpack_dual(y)
+            assert torch.equal(value, want) and torch.equal(slope, moved)
+            if grad_needed:
+                (g,) = torch.autograd.grad((y * y).sum(), leaf)
+                g, dg = forward_ad.unpack_dual(g)
+                assert torch.equal(g, embedding.lookup_gradient(2 * want, index, 40, **how))
+                assert torch.equal(dg, embedding.lookup_gradient(2 * moved, index, 40, **how))
+            plain = embedding.lookup(table, index, **how)
+            assert torch.equal(plain, want) and forward_ad.unpack_dual(plain).tangent is None
