@@ -833,3 +833,62 @@ def test_forward_mode_derivatives(cuda, offset_on_device):
                 assert torch.equal(dg, embedding.lookup_gradient(2 * moved, index, 40, **how))
             plain = embedding.lookup(table, index, **how)
             assert torch.equal(plain, want) and forward_ad.unpack_dual(plain).tangent is None
+
+
+def _sums(terms, index, rows):
+    """Sums of terms by row in 64 bits; exact for whole numbers."""
+    return torch.zeros(rows, terms.shape[1], dtype=torch.float64, device=terms.device).index_add_(
+        0, index, terms)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,rows,width,gap", [(300_000, 17, 5, 0), (100_003, 4096, 48, 0),
+                                              (65_000, 3, 20, 1), (9000, 3, 513, 0),
+                                              (40_000, 700, 64, 8), (20_011, 5, 1, 0)])
+@pytest.mark.parametrize("p", [0.0, 0.5])
+def test_sums_of_whole_numbers_are_exact(cuda, dtype, n, rows, width, gap, p):
+    """Whole numbers up to 4 times the factor of 2 or 1: every sum of them and of
+    any part is a whole number below 2^24, so 32 bits hold it in any order. One
+    token lost, repeated or given to another row shows, however long the row:
+    rows in many groups and blocks, aligned, strided and odd, through the
+    dropout, to the gradient and to Adam (whose first moment, from zero, is the
+    gradient times 1 - 0.9 rounded once)."""
+    import embedding
+
+    whole = torch.randint(-4, 5, (n, width + gap), device=cuda,
+                          generator=torch.Generator(device=cuda).manual_seed(n)).to(dtype)
+    grad = whole[:, :width]
+    terms = grad.double()
+    if p > 0:
+        terms = terms * torch.from_numpy(draws.weight(grad.shape, p, SEED, OFFSET)).to(cuda)
+    for kind in ("skewed", "same", "uniform"):
+        index = torch.from_numpy(_tokens(kind, n, rows, np.random.default_rng(n))).to(cuda)
+        want = _sums(terms, index, rows)
+        got = embedding.lookup_gradient(grad, index, rows, p=p, seed=SEED, offset=OFFSET)
+        assert torch.equal(got, want.to(dtype))
+        table, first, second = (torch.zeros(rows, width, device=cuda) for _ in range(3))
+        embedding.consume_torch_adam(table, first, second, grad, index, rate=0.1, bias1=0.5,
+                                     bias2_sqrt=0.5, p=p, seed=SEED, offset=OFFSET)
+        assert torch.equal(first, ((1.0 - 0.9) * want).float())
+
+
+@pytest.mark.parametrize("width", [1, 5, 8])
+def test_a_row_of_a_million_terms(cuda, width):
+    """The error of a long sum of positive terms. A block adds 3584 terms at most
+    in 32 bits: t a group (t x groups = 3584 at most), the groups' sums eight at
+    a time, their sums in a row; blocks meet in 64 bits. A rounding is off by at
+    most 2^-24 of the sum it rounds, so with terms below one the squares of a
+    block's errors add up to (2^-24)^2 times at most 3584 t^2 + groups (8 t)^2 +
+    groups / 8 x 3584^2, below 29000^2 for 8 to 256 groups. Roundings of terms
+    that know nothing of each other are as good as independent: six times the
+    root of the squares' sum over all blocks is passed with a probability of
+    2 exp(-18) (Hoeffding). The result's own rounding comes on top."""
+    import embedding
+
+    n = 1_100_000
+    grad = torch.rand(n, width, device=cuda,
+                      generator=torch.Generator(device=cuda).manual_seed(width)) / 2 + 0.5
+    got = embedding.lookup_gradient(grad, torch.zeros(n, dtype=torch.int32, device=cuda), 1)
+    want = grad.double().sum(0, keepdim=True)
+    blocks = -(-n // 3584)
+    assert ((got - want).abs() <= 6 * math.sqrt(blocks) * 29_000 * U + want * U).all()
