@@ -1082,8 +1082,11 @@ extern "C" int clad3dgs_describe(int* sm_count, int* tile_gaussians,
 }
 
 extern "C" int clad3dgs_fault_status(int clear, unsigned int* fault_word) {
+  // (A copy from the legacy stream alone waits for no non-blocking stream.)
+  cudaError_t e = cudaDeviceSynchronize();
+  if (e != cudaSuccess) return status_of(e, "waiting for the device");
   unsigned int word = 0;
-  cudaError_t e = cudaMemcpyFromSymbol(&word, g_fault_word, sizeof(word));
+  e = cudaMemcpyFromSymbol(&word, g_fault_word, sizeof(word));
   if (e != cudaSuccess) return status_of(e, "reading the fault word");
   if (clear && word) {
     const unsigned int zero = 0;

@@ -129,7 +129,8 @@ int clad3dgs_describe(int* sm_count, int* tile_gaussians, int* sh_stages,
 
 /* Reads (and clears if clear != 0) the device fault word that bounded waits
  * set when a pipeline barrier timed out, and the table operators (bit 256) when
- * a token's index lay outside its table. 0 means no fault. Synchronises. */
+ * a token's index lay outside its table. 0 means no fault. Waits for all work on
+ * the current device first. */
 int clad3dgs_fault_status(int clear, unsigned int* fault_word);
 
 /* Same as sh_consumer_split_torch_adam with an explicit stream. */

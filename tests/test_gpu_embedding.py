@@ -892,3 +892,29 @@ def test_a_row_of_a_million_terms(cuda, width):
     want = grad.double().sum(0, keepdim=True)
     blocks = -(-n // 3584)
     assert ((got - want).abs() <= 6 * math.sqrt(blocks) * 29_000 * U + want * U).all()
+
+
+def test_bad_indices_are_seen_behind_work_on_another_stream(cuda):
+    """Reading the fault word waits for the device, also for streams that do not
+    wait for the legacy one; all three types and every operator report there."""
+    import _native as native
+    import embedding
+
+    native.fault_status()
+    side = torch.cuda.Stream()
+    bad = torch.full((300,), 9, device=cuda)
+    for dtype in TYPES:
+        table = torch.ones(4, 8, dtype=dtype, device=cuda)
+        grad = torch.ones(300, 8, dtype=dtype, device=cuda)
+        state = _adam_state(4, 8, cuda)
+        for call in (lambda: embedding.lookup(table, bad),
+                     lambda: embedding.lookup_gradient(grad, bad, 4),
+                     lambda: embedding.lookup_gradient(grad[:20], bad[:20], 4),
+                     lambda: embedding.token_order(bad, 4),
+                     lambda: embedding.consume_torch_adam(*state, grad, bad, rate=0.1, bias1=0.5,
+                                                          bias2_sqrt=0.5)):
+            torch.cuda.synchronize()
+            with torch.cuda.stream(side):
+                torch.cuda._sleep(20_000_000)  # about 10 ms
+                call()
+            assert native.fault_status() == 256 and native.fault_status() == 0
