@@ -26,22 +26,15 @@
 #include "token_order.cuh"
 
 namespace clad3dgs {
-int fail(int code, const std::string& message);  // gaussian_step.cu
+// gaussian_step.cu
+int fail(int code, const std::string& message);
+cudaError_t fault_word(unsigned** word);
 
 namespace sums {
 CLAD3DGS_ROW_SUMS(extern, float)           // row_sums_f32.cu
 CLAD3DGS_ROW_SUMS(extern, __half)          // row_sums_f16.cu
 CLAD3DGS_ROW_SUMS(extern, __nv_bfloat16)   // row_sums_bf16.cu
 }  // namespace sums
-
-// Reads (and clears) the words set by indices outside their table.
-cudaError_t token_fault(bool clear, unsigned* word) {
-  cudaError_t e = tokens::take_token_fault(clear, word);
-  if (e == cudaSuccess) e = sums::take_fault<float>(clear, word);
-  if (e == cudaSuccess) e = sums::take_fault<__half>(clear, word);
-  if (e == cudaSuccess) e = sums::take_fault<__nv_bfloat16>(clear, word);
-  return e;
-}
 
 namespace {
 
@@ -95,7 +88,7 @@ __global__ void __launch_bounds__(kThreads)
         v[u] = *reinterpret_cast<const Vec<T, V>*>(table + row * table_stride + column[u]);
     }
   }
-  tokens::report(bad);
+  tokens::report(index, bad);
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const Number at = first + u * kThreads;
@@ -155,7 +148,7 @@ __global__ void __launch_bounds__(kThreads)
       else if (j >= from && j < count) v.v[j] = there[j];
     }
   }
-  tokens::report(bad);
+  tokens::report(index, bad);
   bool keep[V];
   if (kDrop) mask_vector<V, Number>(mask, offset, uint64_t(at), keep);
   v = finish<T, V, kDrop>(v, keep, factor);
@@ -330,7 +323,8 @@ extern "C" int clad3dgs_token_order(int64_t n, int64_t rows, const void* index, 
   if (uint64_t(workspace) % 256 || uint64_t(order) % 8)
     return refuse(what, "unaligned workspace or order");
   if (workspace_bytes < need) return refuse(what, "workspace too small");
-  const tokens::Index x{index, index_bits == 64, has_padding != 0, padding, rows};
+  tokens::Index x{index, index_bits == 64, has_padding != 0, padding, rows};
+  if (const cudaError_t e = fault_word(&x.fault); e != cudaSuccess) return status(what, e);
   return status(what, tokens::sort_tokens(n, x, reinterpret_cast<uint2*>(order), workspace,
                                           tokens::Fill{}, stream));
 }
@@ -347,7 +341,8 @@ extern "C" int clad3dgs_embedding_lookup(int type, int64_t n, int64_t rows, int6
   if (n == 0 || width == 0) return CLAD3DGS_OK;
   if ((!table && rows > 0) || !index || !out) return refuse(what, "null array");
   if (table_stride < 0) return refuse(what, "bad row stride");
-  const tokens::Index x{index, index_bits == 64, has_padding != 0, padding, rows};
+  tokens::Index x{index, index_bits == 64, has_padding != 0, padding, rows};
+  if (const cudaError_t e = fault_word(&x.fault); e != cudaSuccess) return status(what, e);
   const Lookup a{n, width, table, table_stride, x, factor_of(scale, p),
                  counter_mask(p, seed, offset, reinterpret_cast<const long long*>(offset_device)),
                  p > 0.0, out, stream};
@@ -375,10 +370,12 @@ extern "C" int clad3dgs_embedding_gradient(int type, int64_t n, int64_t rows, in
   const char* what = "embedding gradient";
   if (const char* why = problem(n, rows, width, type, scale, p)) return refuse(what, why);
   if (rows == 0 || width == 0) return CLAD3DGS_OK;
-  const Tokens tokens{n, rows, width, Index{index, index_bits == 64, has_padding != 0, padding, rows},
+  Tokens tokens{n, rows, width, Index{index, index_bits == 64, has_padding != 0, padding, rows},
                       index_bits, order, static_cast<char*>(workspace), workspace_bytes};
   if (const char* why = tokens.problem(grad, grad_stride, false)) return refuse(what, why);
   if (!out) return refuse(what, "null array");
+  if (const cudaError_t e = fault_word(&tokens.index.fault); e != cudaSuccess)
+    return status(what, e);
   const CounterMask mask =
       counter_mask(p, seed, offset, reinterpret_cast<const long long*>(offset_device));
   auto go = [&](auto zero) {
@@ -405,10 +402,12 @@ extern "C" int clad3dgs_embedding_consume_torch_adam(
         config.bias2_sqrt > 0.f && config.bias2_sqrt <= 1.f))
     return refuse(what, "invalid Adam configuration");
   if (rows == 0 || width == 0) return CLAD3DGS_OK;
-  const Tokens tokens{n, rows, width, Index{index, index_bits == 64, has_padding != 0, padding, rows},
+  Tokens tokens{n, rows, width, Index{index, index_bits == 64, has_padding != 0, padding, rows},
                       index_bits, order, static_cast<char*>(workspace), workspace_bytes};
   if (const char* why = tokens.problem(grad, grad_stride, true)) return refuse(what, why);
   if (!table || !first || !second) return refuse(what, "null array");
+  if (const cudaError_t e = fault_word(&tokens.index.fault); e != cudaSuccess)
+    return status(what, e);
   const sums::Adam adam{table, first, second, float(rate / double(config.bias1)),
                         1.0 / double(config.bias2_sqrt)};
   const CounterMask mask =

@@ -781,7 +781,17 @@ __global__ void quaternion_kernel(long long n, const float* __restrict__ q,
 // ---------------------------------------------------------------------------
 // Host side.
 
-cudaError_t token_fault(bool clear, unsigned* word);  // embedding.cu
+// The current device's fault word, for the kernels of other files. The first call
+// may be under a stream capture, which the loading of the module must not
+// disturb. (About 100 ns; an address kept would be wrong after a device reset.)
+cudaError_t fault_word(unsigned** word) {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e != cudaSuccess) return e;
+  e = cudaGetSymbolAddress(reinterpret_cast<void**>(word), g_fault_word);
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  return e;
+}
 
 thread_local std::string t_last_error;
 
@@ -1093,13 +1103,11 @@ extern "C" int clad3dgs_fault_status(int clear, unsigned int* fault_word) {
     e = cudaMemcpyToSymbol(g_fault_word, &zero, sizeof(zero));
     if (e != cudaSuccess) return status_of(e, "clearing the fault word");
   }
-  unsigned int token_word = 0;
-  e = token_fault(clear != 0, &token_word);
-  if (e != cudaSuccess) return status_of(e, "reading the token fault word");
-  if (fault_word) *fault_word = word | token_word;
-  if (word) return fail(CLAD3DGS_DEVICE_FAULT, "a pipeline wait timed out");
-  return token_word ? fail(CLAD3DGS_DEVICE_FAULT, "a token's index lay outside its table")
-                    : CLAD3DGS_OK;
+  if (fault_word) *fault_word = word;
+  if (word & (kFaultProducerWait | kFaultConsumerWait))
+    return fail(CLAD3DGS_DEVICE_FAULT, "a pipeline wait timed out");
+  return word ? fail(CLAD3DGS_DEVICE_FAULT, "a token's index lay outside its table")
+              : CLAD3DGS_OK;
 }
 
 extern "C" int clad3dgs_sh_consume_split_torch_adam(

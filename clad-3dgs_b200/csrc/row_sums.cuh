@@ -679,7 +679,7 @@ __global__ void __launch_bounds__(kFewThreads)
     bool bad = false;
     const uint32_t key =
         me < n ? tokens::row_of(index, tokens::raw_index(index, me), &bad) : kNoRow;
-    tokens::report(bad);
+    tokens::report(index, bad);
     if (me < n) keys[me] = key;
     __syncthreads();
     if (me < n) {
@@ -893,19 +893,12 @@ cudaError_t consume(const Args<T>& a, const tokens::Index& index, const Adam& ad
   return run(a.rows, a.width, a.n > 0 ? kept.slots : nullptr, kept.sums, adam, stream);
 }
 
-// The fault word of the file that holds T's kernels.
-template <class T>
-cudaError_t take_fault(bool clear, unsigned* word) {
-  return tokens::take_token_fault(clear, word);
-}
-
 // The kernels of each element type are compiled in a file of their own.
 #define CLAD3DGS_ROW_SUMS(prefix, T)                                                      \
   prefix template cudaError_t gradient<T>(const Args<T>&, const tokens::Index&, T*, bool,  \
                                           cudaStream_t);                                   \
   prefix template cudaError_t consume<T>(const Args<T>&, const tokens::Index&, const Adam&, \
-                                         bool, cudaStream_t);                              \
-  prefix template cudaError_t take_fault<T>(bool, unsigned*);
+                                         bool, cudaStream_t);
 
 }  // namespace sums
 }  // namespace clad3dgs

@@ -7,10 +7,9 @@
 namespace clad3dgs {
 namespace tokens {
 
-// Set when a kernel met an index outside its table that is not the padding: a
-// word in every file that includes this, read by take_token_fault.
+// Set in the fault word when a kernel met an index outside its table that is not
+// the padding.
 constexpr unsigned kFaultTokenRange = 256u;
-static __device__ unsigned int g_token_fault = 0;
 
 // The indices a caller gives.
 struct Index {
@@ -19,6 +18,7 @@ struct Index {
   bool has_padding;
   int64_t padding;
   int64_t rows;
+  unsigned* fault = nullptr;  // the device's fault word, for kernels that read indices
 };
 
 __device__ __forceinline__ int64_t raw_index(const Index& x, int64_t i) {
@@ -37,20 +37,8 @@ __device__ __forceinline__ uint32_t row_of(const Index& x, int64_t t, bool* bad)
 
 // Once a thread, for all its indices: an atomic between two of them would hold
 // back the loads behind it.
-__device__ __forceinline__ void report(bool bad) {
-  if (bad) atomicOr(&g_token_fault, kFaultTokenRange);
-}
-
-// Adds this file's fault word to *word, and clears it if asked to.
-static inline cudaError_t take_token_fault(bool clear, unsigned* word) {
-  unsigned mine = 0;
-  cudaError_t e = cudaMemcpyFromSymbol(&mine, g_token_fault, sizeof(mine));
-  if (e == cudaSuccess && clear && mine) {
-    const unsigned zero = 0;
-    e = cudaMemcpyToSymbol(g_token_fault, &zero, sizeof(zero));
-  }
-  *word |= mine;
-  return e;
+__device__ __forceinline__ void report(const Index& x, bool bad) {
+  if (bad) atomicOr(x.fault, kFaultTokenRange);
 }
 
 }  // namespace tokens

@@ -48,7 +48,7 @@ __device__ __forceinline__ void load_pairs(const Index& index, const uint2* from
 #pragma unroll
   for (int j = 0; j < I; ++j)
     if (at(j) < n) pair[j] = make_uint2(row_of(index, raw[j], &bad), uint32_t(at(j)));
-  report(bad);
+  report(index, bad);
 }
 
 // Ranks of a tile: thread t of warp w holds the tokens w * 32 * I + 32 * j + lane,

@@ -127,10 +127,11 @@ const char* clad3dgs_last_error(void);
 int clad3dgs_describe(int* sm_count, int* tile_gaussians, int* sh_stages,
                       int* fused_stages);
 
-/* Reads (and clears if clear != 0) the device fault word that bounded waits
- * set when a pipeline barrier timed out, and the table operators (bit 256) when
- * a token's index lay outside its table. 0 means no fault. Waits for all work on
- * the current device first. */
+/* Reads (and clears if clear != 0) the current device's fault word: bits 1 and 2
+ * are set by bounded waits that gave up on a pipeline barrier, bit 256 by the
+ * table operators when a token's index lay outside its table. 0 means no fault;
+ * CLAD3DGS_DEVICE_FAULT is returned for any bit. Waits for all work on the
+ * device first. Kernels report to the device they ran on: make it current. */
 int clad3dgs_fault_status(int clear, unsigned int* fault_word);
 
 /* Same as sh_consumer_split_torch_adam with an explicit stream. */

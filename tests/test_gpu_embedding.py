@@ -918,3 +918,54 @@ def test_bad_indices_are_seen_behind_work_on_another_stream(cuda):
                 torch.cuda._sleep(20_000_000)  # about 10 ms
                 call()
             assert native.fault_status() == 256 and native.fault_status() == 0
+
+
+def test_first_call_of_a_process_under_capture(cuda):
+    """A process whose first call of the library is captured into a graph."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    code = """
+import sys
+sys.path.insert(0, sys.argv[1])
+import torch
+import _native as native
+import embedding
+table = torch.arange(32.0, device="cuda").view(8, 4)
+index = torch.tensor([3, 9, 7], device="cuda")
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = embedding.lookup(table, index)
+    g = embedding.lookup_gradient(y, index, 8)
+graph.replay()
+torch.cuda.synchronize()
+assert y.tolist() == [table[3].tolist(), [0.0] * 4, table[7].tolist()]
+assert g[3].tolist() == table[3].tolist() and g[7].tolist() == table[7].tolist()
+assert native.fault_status() == 256
+"""
+    package = Path(__file__).resolve().parents[1] / "clad-3dgs_b200"
+    run = subprocess.run([sys.executable, "-c", code, str(package)], capture_output=True, text=True,
+                         timeout=300)
+    assert run.returncode == 0, run.stderr[-2000:]
+
+
+def test_reading_the_fault_word_clears_it_or_leaves_it(cuda):
+    """One word for all operators: without `clear` its bits stay for the next
+    reader, and the status says what it holds."""
+    import ctypes
+
+    import _native as native
+    import embedding
+
+    native.fault_status()
+    word = ctypes.c_uint(7)
+    status = lambda clear: native.library().clad3dgs_fault_status(clear, ctypes.byref(word))
+    assert status(0) == native.OK and word.value == 0
+    table, bad = torch.ones(4, 8, dtype=torch.float16, device=cuda), torch.full((3,), 4, device=cuda)
+    embedding.lookup(table, bad)
+    embedding.lookup_gradient(table[:3], bad, 4)
+    for clear in (0, 0, 1):
+        assert status(clear) == native.DEVICE_FAULT and word.value == 256
+        assert b"index" in native.library().clad3dgs_last_error()
+    assert status(1) == native.OK and word.value == 0
