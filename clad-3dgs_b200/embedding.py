@@ -44,6 +44,7 @@ from dropout import TYPES, check_draw, launch
 
 MOST = 2 ** 31 - 1
 _BITS = {torch.int32: 32, torch.int64: 64}
+_LARGEST = torch.finfo(torch.float32).max
 
 
 def _require(condition, message):
@@ -59,6 +60,7 @@ class TokenOrder(NamedTuple):
 
 def _index(index, device):
     """The checked index: (tensor, bits)."""
+    _require(isinstance(index, torch.Tensor), "index must be a tensor")
     _require(index.is_cuda and (device is None or index.device == device),
              "index must be on the tensors' CUDA device")
     bits = _BITS.get(index.dtype)
@@ -75,8 +77,11 @@ def _padding(padding_index):
     return 1, padding_index
 
 
-def _check_scale(scale):
-    _require(isinstance(scale, (int, float)) and abs(scale) <= 1e38, "scale must be finite")
+def _check_scale(scale, p):
+    """p as `check_draw` leaves it."""
+    _require(isinstance(scale, (int, float)) and abs(scale) <= 1e38
+             and (p == 1 or abs(scale) / (1 - p) <= _LARGEST),
+             "scale and scale / (1 - p) must be finite in 32 bits")
 
 
 def _check_rows(rows):
@@ -154,12 +159,12 @@ def _workspace(count, rows, width, consume, ordered, like):
 def _lookup(table, index, scale, padding_index, p, seed, offset):
     table, kind, rows, width, stride = _matrix(table, "table")
     device = table.device
-    shape = (*index.shape, width)
     index, bits = _index(index, device)
+    shape = (*index.shape, width)
     _check_rows(rows)
-    _check_scale(scale)
     padded, padding = _padding(padding_index)
     number, address = check_draw(p, seed, offset, device)
+    _check_scale(scale, p)
     out = table.new_empty(shape)
     if out.numel():
         launch(device, "embedding lookup", native.library().clad3dgs_embedding_lookup, kind,
@@ -182,8 +187,8 @@ def lookup_gradient(grad, index, rows, *, scale=1.0, padding_index=None, p=0.0, 
     grad, kind, count, width, stride = _gradient_matrix(grad)
     device = grad.device
     _check_rows(rows)
-    _check_scale(scale)
     number, address = check_draw(p, seed, offset, device)
+    _check_scale(scale, p)
     tokens, alive = _tokens(index, rows, padding_index, order, count, device)
     out = grad.new_empty((rows, width))
     if out.numel():
@@ -213,10 +218,11 @@ def consume_torch_adam(table, first, second, grad, index, *, rate, bias1, bias2_
                  "[rows, width] on grad's device")
     _require(shape[1] == width, "table and grad must have the same width")
     _check_rows(rows)
-    _check_scale(scale)
-    _require(math.isfinite(rate) and rate >= 0 and 0 < bias1 <= 1 and 0 < bias2_sqrt <= 1,
-             "invalid Adam configuration")
+    config = native.TorchAdamConfig(bias1, bias2_sqrt)  # (rounds to 32 bits)
+    _require(math.isfinite(rate) and rate >= 0 and bias1 <= 1 and bias2_sqrt <= 1
+             and config.bias1 > 0 and config.bias2_sqrt > 0, "invalid Adam configuration")
     number, address = check_draw(p, seed, offset, device)
+    _check_scale(scale, p)
     tokens, alive = _tokens(index, rows, padding_index, order, count, device)
     size = 4 * rows * width
     spans = [(t.data_ptr(), t.data_ptr() + size) for t in state]
@@ -232,17 +238,18 @@ def consume_torch_adam(table, first, second, grad, index, *, rate, bias1, bias2_
         launch(device, "embedding consume", native.library().clad3dgs_embedding_consume_torch_adam,
                kind, count, rows, width, grad.data_ptr(), stride, *tokens, scale, p, seed, number,
                address, spans[0][0], spans[1][0], spans[2][0], rate,
-               native.TorchAdamConfig(bias1, bias2_sqrt), space[1], space[2])
+               config, space[1], space[2])
 
 
 class _Lookup(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, index, scale, padding_index, p, seed, offset, order):
+        out = _lookup(table, index, scale, padding_index, p, seed, offset)
         tensor = isinstance(offset, torch.Tensor)
         ctx.numbers = (table.shape[0], scale, padding_index, p, seed, None if tensor else offset,
                        order)
         ctx.save_for_backward(index, *((offset,) if tensor else ()))
-        return _lookup(table, index, scale, padding_index, p, seed, offset)
+        return out
 
     @staticmethod
     def backward(ctx, grad):
@@ -266,6 +273,8 @@ def lookup(table, index, *, scale=1.0, padding_index=None, p=0.0, seed=0, offset
         return make_dual(lookup(primal, index, **how), lookup(tangent, index, **how))
     if table.requires_grad and torch.is_grad_enabled():
         if order is not None:
+            _require(table.dim() == 2 and isinstance(index, torch.Tensor),
+                     "table must be a matrix and index a tensor")
             _tokens(None, table.shape[0], None, order, index.numel(), table.device)
         return _Lookup.apply(table, index, scale, padding_index, p, seed, offset, order)
     return _lookup(table, index, scale, padding_index, p, seed, offset)

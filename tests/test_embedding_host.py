@@ -115,3 +115,26 @@ def test_workspaces():
     sizes = [lib.clad3dgs_embedding_workspace(n, rows, 48, 1, 0) > 0
              for n, rows in ((128, 1365), (128, 1366), (256, 682), (256, 683), (257, 1))]
     assert sizes == [False, True, False, True, True]
+
+
+@pytest.mark.parametrize("scale,p,fits", [
+    (1.0, 0.0, True), (-2, 0.5, True), (1e38, 0.5, True), (1e38, 1, True), (1e38, 1.0, True),
+    (0.0, 1.0 - 1e-15, True), (1e38, 0.999, False), (-1e38, 0.999, False), (1e39, 0.0, False),
+    (10 ** 400, 0.0, False), (INF, 0.0, False), (NAN, 0.0, False), (NAN, 1.0, False),
+    ("1", 0.0, False), (None, 0.0, False)])
+def test_scales_are_checked(scale, p, fits):
+    import embedding
+
+    if fits:
+        embedding._check_scale(scale, p)
+    else:
+        with pytest.raises(RuntimeError, match="scale"):
+            embedding._check_scale(scale, p)
+
+
+def test_an_index_has_to_be_a_tensor():
+    import embedding
+
+    for index in (None, [0, 1]):
+        with pytest.raises(RuntimeError, match="index"):
+            embedding.token_order(index, 4)

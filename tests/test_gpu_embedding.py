@@ -969,3 +969,37 @@ def test_reading_the_fault_word_clears_it_or_leaves_it(cuda):
         assert status(clear) == native.DEVICE_FAULT and word.value == 256
         assert b"index" in native.library().clad3dgs_last_error()
     assert status(1) == native.OK and word.value == 0
+
+
+def test_what_only_the_library_could_refuse_is_a_runtime_error(cuda):
+    """Factors and bias corrections that do not fit 32 bits, and tables and
+    indices that are none."""
+    import embedding
+
+    table, index, grad = _case(10, 4, 6, torch.float32, cuda)
+    state = _adam_state(4, 6, cuda)
+    adam = dict(rate=0.1, bias1=0.5, bias2_sqrt=0.5)
+    before = [t.clone() for t in state]
+    leaf = torch.ones((), device=cuda, requires_grad=True)
+    for call in (lambda: embedding.lookup(table, index, scale=1e38, p=0.999),
+                 lambda: embedding.lookup(table, index, scale=1e39),
+                 lambda: embedding.lookup_gradient(grad, index, 4, scale=-1e38, p=0.999),
+                 lambda: embedding.consume_torch_adam(*state, grad, index, **adam, scale=1e38,
+                                                      p=0.999),
+                 lambda: embedding.consume_torch_adam(*state, grad, index, **{**adam, "bias1": 1e-50}),
+                 lambda: embedding.consume_torch_adam(*state, grad, index,
+                                                      **{**adam, "bias2_sqrt": 1e-50}),
+                 lambda: embedding.lookup_gradient(grad, None, 4),
+                 lambda: embedding.lookup(table, [0, 1]),
+                 lambda: embedding.lookup(table.clone().requires_grad_(True), [0, 1]),
+                 lambda: embedding.lookup(table.clone().requires_grad_(True), None,
+                                          order=embedding.token_order(index, 4)),
+                 lambda: embedding.lookup(leaf, index),
+                 lambda: embedding.lookup(leaf.detach(), index),
+                 lambda: embedding.lookup(leaf, index, order=embedding.token_order(index, 4))):
+        with pytest.raises(RuntimeError):
+            call()
+    assert all(torch.equal(a, b) for a, b in zip(state, before))
+    # A factor near the largest number is none of them.
+    assert torch.isfinite(embedding.lookup(torch.full((4, 6), 0.5, device=cuda), index,
+                                           scale=1e38, p=0.5)).all()
