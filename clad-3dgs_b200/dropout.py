@@ -93,14 +93,18 @@ def _check(x, p, seed, offset):
 
 def apply(x, p, seed, offset=0, *, rows=False, out=None):
     """The dropout without autograd. `out`: a contiguous tensor like x to write
-    into; x itself (contiguous) for a call in place."""
+    into; x itself (contiguous) for a call in place. Its autograd version is
+    counted up, so a backward pass that needs its old values is refused."""
     number, address = _check(x, p, seed, offset)
     if out is not None:
         _require(out.device == x.device and out.dtype == x.dtype and out.shape == x.shape
                  and out.is_contiguous(), "out must be a contiguous tensor like x")
         same = out.data_ptr() == x.data_ptr() and x.is_contiguous()
         _require(same or not overlap(x, out), "out may be x itself, but not overlap it otherwise")
-    return _run(x.detach(), p, seed, number, address, bool(rows), out)
+    y = _run(x.detach(), p, seed, number, address, bool(rows), out)
+    if out is not None and not out.is_inference():
+        torch.autograd.graph.increment_version(out)
+    return y
 
 
 def overlap(x, y):

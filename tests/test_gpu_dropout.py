@@ -246,3 +246,29 @@ def test_forward_mode_derivatives(cuda, rows, offset_on_device):
                 g, dg = forward_ad.unpack_dual(g)
                 assert torch.equal(g, drop(2 * want)) and torch.equal(dg, drop(2 * moved))
             assert forward_ad.unpack_dual(drop(x)).tangent is None
+
+
+def test_writing_into_a_saved_tensor_is_seen_by_autograd(cuda):
+    """`out` is written in place: a backward pass that needs its old values is
+    refused, as after torch's own operations in place."""
+    import dropout
+
+    for place in (lambda x: dropout.apply(x, 0.5, 1, 2, out=x),
+                  lambda x: dropout.apply(torch.ones_like(x), 0.5, 1, 2, out=x)):
+        w = torch.ones(16, device=cuda, requires_grad=True)
+        x = torch.full((16,), 3.0, device=cuda)
+        y = (w * x).sum()
+        place(x)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+
+
+def test_writing_into_an_inference_tensor(cuda):
+    import dropout
+
+    x = _input((9, 5), torch.float32, cuda)
+    with torch.inference_mode():
+        out = torch.empty(9, 5, device=cuda)
+        assert torch.equal(dropout.apply(x, 0.5, 1, 2, out=out), dropout.apply(x, 0.5, 1, 2))
+        dropout.apply(x, 0.5, 1, 2, out=x)
+        assert torch.equal(x, out)
