@@ -62,7 +62,7 @@ __device__ __forceinline__ Vec<T, V> finish(const Vec<T, V>& x, const bool (&kee
 template <class T, class Division, int V, int U, bool kDrop>
 __global__ void __launch_bounds__(kThreads)
     lookup_kernel(typename Division::Number total, const Division vectors,
-                  const T* __restrict__ table, int64_t table_stride, Index index, float factor,
+                  const T* table, int64_t table_stride, Index index, float factor,
                   const __grid_constant__ CounterMask mask, T* __restrict__ out) {
   using Number = typename Division::Number;
   wait_before();
@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(kThreads)
 template <class T, class Division, int V, bool kShort, bool kDrop>
 __global__ void __launch_bounds__(kThreads)
     lookup_odd_kernel(typename Division::Number total, const Division width,
-                      const T* __restrict__ table, int64_t table_stride, Index index,
+                      const T* table, int64_t table_stride, Index index,
                       float factor, const __grid_constant__ CounterMask mask,
                       T* __restrict__ out) {
   using Number = typename Division::Number;

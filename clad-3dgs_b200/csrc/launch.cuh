@@ -7,6 +7,10 @@
 // block passes it, so a kernel's end means that all kernels before it have
 // ended too, and memory may be reused along the stream as usual. Behind
 // anything but a kernel of this kind the launch is an ordinary one.
+//
+// Such a kernel's pointers to what earlier kernels write are not `const
+// __restrict__`: that would promise that the data does not change while the
+// kernel runs (reads through the read-only path), and it runs before they end.
 #pragma once
 #include <cuda_runtime.h>
 

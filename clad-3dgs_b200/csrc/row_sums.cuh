@@ -580,7 +580,7 @@ struct Adam {
 template <class Division, int W, int U>
 __global__ void __launch_bounds__(kThreads)
     adam_kernel(typename Division::Number total, const Division vectors, int64_t width,
-                const int32_t* __restrict__ slots, const float* __restrict__ sums, const Adam a) {
+                const int32_t* slots, const float* sums, const Adam a) {
   wait_before();
   using Number = typename Division::Number;
   using F = Vec<float, W>;

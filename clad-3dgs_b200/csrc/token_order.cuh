@@ -291,7 +291,7 @@ inline SortPlan sort_plan(int64_t n, int64_t rows) {
 // counts[block][digit]
 template <int I>
 __global__ void __launch_bounds__(kSortThreads)
-    count_kernel(int64_t n, Index index, const uint2* __restrict__ from, int tiles, int shift,
+    count_kernel(int64_t n, Index index, const uint2* from, int tiles, int shift,
                  int bits, uint32_t* __restrict__ counts, const Fill fill) {
   wait_before();
   fill.run();
@@ -314,8 +314,8 @@ __global__ void __launch_bounds__(kSortThreads)
 
 template <int I>
 __global__ void __launch_bounds__(kSortThreads)
-    scatter_kernel(int64_t n, Index index, const uint2* __restrict__ from, int tiles, int shift,
-                   int bits, const uint32_t* __restrict__ counts, uint2* __restrict__ to) {
+    scatter_kernel(int64_t n, Index index, const uint2* from, int tiles, int shift,
+                   int bits, const uint32_t* counts, uint2* __restrict__ to) {
   wait_before();
   extern __shared__ __align__(16) char shared[];
   const int digits = 1 << bits;

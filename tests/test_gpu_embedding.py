@@ -1003,3 +1003,29 @@ def test_what_only_the_library_could_refuse_is_a_runtime_error(cuda):
     # A factor near the largest number is none of them.
     assert torch.isfinite(embedding.lookup(torch.full((4, 6), 0.5, device=cuda), index,
                                            scale=1e38, p=0.5)).all()
+
+
+@pytest.mark.parametrize("n,rows", [(3000, 300_000), (40_000, 300_000), (40_000, 2000)])
+def test_sorts_back_to_back(cuda, n, rows):
+    """Passes and calls that overwrite the same memory one after the other, all in
+    flight at once: every call sees its own passes' counts and pairs, and every
+    update the sums of its own step."""
+    import embedding
+
+    g = torch.Generator(device=cuda).manual_seed(n)
+    indices = [torch.randint(0, rows, (n,), device=cuda, generator=g) for _ in range(60)]
+    grads = [torch.randint(-4, 5, (n, 4), device=cuda, generator=g).float() for _ in indices]
+    torch.cuda.synchronize()
+    first = torch.zeros(rows, 4, device=cuda)
+    state = torch.zeros_like(first), first, torch.zeros_like(first)
+    orders, firsts = [], []
+    for index, grad in zip(indices, grads):
+        orders.append(embedding.token_order(index, rows).pairs)
+        first.zero_()
+        embedding.consume_torch_adam(*state, grad, index, rate=0.1, bias1=0.5, bias2_sqrt=0.5)
+        firsts.append(first[:2000].clone())
+    for index, grad, order, moment in zip(indices, grads, orders, firsts):
+        row, place = torch.sort(index, stable=True)
+        assert torch.equal(order.long(), torch.stack([row, place], dim=1))
+        want = _sums(grad.double(), index, rows)[:2000]
+        assert torch.equal(moment, ((1.0 - 0.9) * want).float())
