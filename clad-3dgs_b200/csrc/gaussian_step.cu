@@ -26,6 +26,7 @@
 //  * The tail tile and inputs that are not 16-byte aligned go through a plain
 //    one-tile-per-CTA kernel with the same arithmetic.
 #include <algorithm>
+#include <atomic>
 #include <cstdint>
 #include <cstdio>
 #include <cstring>
@@ -781,15 +782,24 @@ __global__ void quaternion_kernel(long long n, const float* __restrict__ q,
 // ---------------------------------------------------------------------------
 // Host side.
 
-// The current device's fault word, for the kernels of other files. The first call
-// may be under a stream capture, which the loading of the module must not
-// disturb. (About 100 ns; an address kept would be wrong after a device reset.)
+// The current device's fault word, for the kernels of other files. A device's first
+// call may be under a stream capture, which the loading of the module must not
+// disturb. (The address itself is asked for every time, 34 ns: one kept would be
+// wrong after a device reset.)
 cudaError_t fault_word(unsigned** word) {
-  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-  cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);
+  static std::atomic<bool> loaded[64];
+  void** const at = reinterpret_cast<void**>(word);
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  e = cudaGetSymbolAddress(reinterpret_cast<void**>(word), g_fault_word);
+  if (dev < 64 && loaded[dev].load(std::memory_order_relaxed))
+    return cudaGetSymbolAddress(at, g_fault_word);
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  e = cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e != cudaSuccess) return e;
+  e = cudaGetSymbolAddress(at, g_fault_word);
   cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e == cudaSuccess && dev < 64) loaded[dev].store(true, std::memory_order_relaxed);
   return e;
 }
 

@@ -22,7 +22,7 @@ raise RuntimeError before anything is written.
 from __future__ import annotations
 
 import torch
-from torch.autograd.forward_ad import make_dual, unpack_dual
+from torch.autograd import forward_ad
 
 import _native as native
 
@@ -47,6 +47,14 @@ def check_draw(p, seed, offset, device):
     _require(isinstance(offset, int) and 0 <= offset < WORD,
              "offset must be an integer in [0, 2^64) or a CUDA tensor")
     return offset, None
+
+
+def parts_of(x):
+    """(x without its tangent, the tangent) of a dual tensor, None of another. Only
+    within a dual level there are any (forward_ad._current_level, -1 outside);
+    callers look at that first, for asking torch takes 0.5 us."""
+    primal, tangent = forward_ad.unpack_dual(x)
+    return None if tangent is None else (primal, tangent)
 
 
 def row_layout(x):
@@ -132,7 +140,7 @@ class _Dropout(torch.autograd.Function):
         p, seed, offset, rows = ctx.numbers
         if offset is None:
             offset = ctx.saved_tensors[0]
-        elif not torch.is_grad_enabled() and unpack_dual(grad).tangent is None:
+        elif not torch.is_grad_enabled() and forward_ad._current_level < 0:
             return _run(grad, p, seed, offset, None, rows), None, None, None, None
         return dropout(grad, p, seed, offset, rows=rows), None, None, None, None
 
@@ -141,10 +149,8 @@ def dropout(x, p, seed, offset=0, *, rows=False):
     """x with a share p of its elements (rows=True: of its rows) set to zero and
     the others scaled by 1 / (1 - p); differentiable any number of times, in
     reverse and in forward mode."""
-    primal, tangent = unpack_dual(x)
-    if tangent is not None:  # the map is linear
-        draw = dict(p=p, seed=seed, offset=offset, rows=rows)
-        return make_dual(dropout(primal, **draw), dropout(tangent, **draw))
+    if forward_ad._current_level >= 0 and (parts := parts_of(x)):  # the map is linear
+        return forward_ad.make_dual(*(dropout(t, p, seed, offset, rows=rows) for t in parts))
     if x.requires_grad and torch.is_grad_enabled():
         return _Dropout.apply(x, p, seed, offset, bool(rows))
     number, address = _check(x, p, seed, offset)

@@ -37,10 +37,10 @@ from functools import lru_cache
 from typing import NamedTuple
 
 import torch
-from torch.autograd.forward_ad import make_dual, unpack_dual
+from torch.autograd import forward_ad
 
 import _native as native
-from dropout import TYPES, check_draw, launch
+from dropout import TYPES, check_draw, launch, parts_of
 
 MOST = 2 ** 31 - 1
 _BITS = {torch.int32: 32, torch.int64: 64}
@@ -60,12 +60,14 @@ class TokenOrder(NamedTuple):
 
 def _index(index, device):
     """The checked index: (tensor, bits)."""
-    _require(isinstance(index, torch.Tensor), "index must be a tensor")
-    _require(index.is_cuda and (device is None or index.device == device),
-             "index must be on the tensors' CUDA device")
+    if not (isinstance(index, torch.Tensor) and index.is_cuda
+            and (device is None or index.device == device)):
+        raise RuntimeError("index must be a tensor on the others' CUDA device")
     bits = _BITS.get(index.dtype)
-    _require(bits is not None, "index must be int32 or int64")
-    _require(index.numel() <= MOST, "at most 2^31 - 1 tokens")
+    if bits is None:
+        raise RuntimeError("index must be int32 or int64")
+    if index.numel() > MOST:
+        raise RuntimeError("at most 2^31 - 1 tokens")
     return index if index.is_contiguous() else index.contiguous(), bits
 
 
@@ -79,9 +81,9 @@ def _padding(padding_index):
 
 def _check_scale(scale, p):
     """p as `check_draw` leaves it."""
-    _require(isinstance(scale, (int, float)) and abs(scale) <= 1e38
-             and (p == 1 or abs(scale) / (1 - p) <= _LARGEST),
-             "scale and scale / (1 - p) must be finite in 32 bits")
+    if not (isinstance(scale, (int, float)) and abs(scale) <= 1e38
+            and (p == 1 or abs(scale) / (1 - p) <= _LARGEST)):
+        raise RuntimeError("scale and scale / (1 - p) must be finite in 32 bits")
 
 
 def _check_rows(rows):
@@ -178,12 +180,10 @@ def lookup_gradient(grad, index, rows, *, scale=1.0, padding_index=None, p=0.0, 
     """The table's gradient [rows, width] (grad's type) of a `lookup` with these
     arguments whose output has the gradient `grad` [*index.shape, width]. With
     `order` (from `token_order`), index and padding_index are not read."""
-    primal, tangent = unpack_dual(grad)
-    if tangent is not None:  # as in lookup
+    if forward_ad._current_level >= 0 and (parts := parts_of(grad)):  # as in lookup
         how = dict(scale=scale, padding_index=padding_index, p=p, seed=seed, offset=offset,
                    order=order)
-        return make_dual(lookup_gradient(primal, index, rows, **how),
-                         lookup_gradient(tangent, index, rows, **how))
+        return forward_ad.make_dual(*(lookup_gradient(t, index, rows, **how) for t in parts))
     grad, kind, count, width, stride = _gradient_matrix(grad)
     device = grad.device
     _check_rows(rows)
@@ -266,11 +266,10 @@ def lookup(table, index, *, scale=1.0, padding_index=None, p=0.0, seed=0, offset
     """scale * table[index], of the table's type, shaped [*index.shape, width]; with
     p > 0 through the dropout of (p, seed, offset). `order` (from `token_order`
     of the same index, rows and padding) spares the backward pass its sort."""
-    primal, tangent = unpack_dual(table)
-    if tangent is not None:  # the map is linear in the table
+    if forward_ad._current_level >= 0 and (parts := parts_of(table)):  # linear in the table
         how = dict(scale=scale, padding_index=padding_index, p=p, seed=seed, offset=offset,
                    order=order)
-        return make_dual(lookup(primal, index, **how), lookup(tangent, index, **how))
+        return forward_ad.make_dual(*(lookup(t, index, **how) for t in parts))
     if table.requires_grad and torch.is_grad_enabled():
         if order is not None:
             _require(table.dim() == 2 and isinstance(index, torch.Tensor),
