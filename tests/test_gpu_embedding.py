@@ -1029,3 +1029,26 @@ def test_sorts_back_to_back(cuda, n, rows):
         assert torch.equal(order.long(), torch.stack([row, place], dim=1))
         want = _sums(grad.double(), index, rows)[:2000]
         assert torch.equal(moment, ((1.0 - 0.9) * want).float())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("p", [0.0, 0.5])
+def test_rows_wider_than_the_gpu_has_places(cuda, dtype, p):
+    """More slices of columns than blocks that run at once: whole numbers, exact."""
+    import embedding
+
+    n, rows = 130, 3
+    for width in (300_000, 300_001):
+        grad = torch.randint(-4, 5, (n, width), device=cuda,
+                             generator=torch.Generator(device=cuda).manual_seed(n)).to(dtype)
+        index = torch.randint(0, rows, (n,), device=cuda,
+                              generator=torch.Generator(device=cuda).manual_seed(1))
+        got = embedding.lookup_gradient(grad, index, rows, p=p, seed=SEED, offset=OFFSET)
+        terms = grad.double()
+        if p > 0:
+            ones = embedding.lookup(torch.ones(1, width, device=cuda), torch.zeros_like(index), p=p,
+                                    seed=SEED, offset=OFFSET)
+            kept = draws.keep(129 * width + np.arange(width - 1000, width), p, SEED, OFFSET)
+            assert np.array_equal(ones[129, -1000:].cpu().numpy(), kept / (1 - p))
+            terms = terms * ones
+        assert torch.equal(got, _sums(terms, index, rows).to(dtype))
