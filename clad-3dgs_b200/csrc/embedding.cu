@@ -418,9 +418,9 @@ extern "C" int clad3dgs_embedding_consume_torch_adam(
     cudaError_t e = cudaSuccess;
     tokens::Fill fill;
     if (n > 0 && !sums::few(n, rows, width)) {
-      // The slots of few rows are cleared by the sort, if there is one.
+      // The slots are cleared by the sort, if there is one and they are few.
       const sums::Kept kept(tokens.partial(), n, rows, width);
-      if (tokens.sorts() && rows <= (1 << 18))
+      if (tokens.sorts() && tokens::sort_clears(n, rows, rows))
         fill = {reinterpret_cast<uint4*>(kept.slots),
                 int64_t(sums::slot_bytes(rows) / sizeof(uint4))};
       else

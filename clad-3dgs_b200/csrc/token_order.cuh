@@ -227,13 +227,22 @@ __global__ void __launch_bounds__(kSortThreads)
   }
 }
 
+// Tokens of a thread, and blocks: as many blocks as give each thread one token,
+// then more tokens a thread.
+inline int cluster_items(int64_t n) { return n <= kSmall / 4 ? 1 : n <= kSmall / 2 ? 2 : 4; }
+
+inline unsigned cluster_blocks(int64_t n) {
+  unsigned blocks = 1;
+  while (int64_t(blocks) * cluster_items(n) * kSortThreads < n) blocks *= 2;
+  return blocks;
+}
+
 template <int I>
 cudaError_t cluster_sort(int64_t n, const Index& index, uint2* order, const Fill& fill,
                          cudaStream_t stream) {
   const int all = key_bits(index.rows);
   const int passes = (all + kDigitBits - 1) / kDigitBits, bits = (all + passes - 1) / passes;
-  unsigned blocks = 1;
-  while (int64_t(blocks) * I * kSortThreads < n) blocks *= 2;
+  const unsigned blocks = cluster_blocks(n);
   constexpr size_t kTileBytes = size_t(I) * kSortThreads * sizeof(uint2);
   const size_t shared = kTileBytes + digit_bytes(bits);
   cudaError_t e = allow_shared(cluster_sort_kernel<I>, kTileBytes + digit_bytes(kDigitBits));
@@ -416,14 +425,27 @@ cudaError_t large_sort(int64_t n, const Index& index, const SortPlan& p, uint2* 
   return cudaSuccess;
 }
 
+// Whether the sort should clear `words` of memory by the way (Fill): its blocks
+// are few, so up to 32768 words each and as many again (Adam's slots, whole calls:
+// 300 tokens and 2^16 rows 22 us against 24 with a launch of its own, 2^18 rows 36
+// against 24; 16000 tokens and 2^18 rows 33 against 34, 2^19 rows 38 against 36;
+// 150000 tokens and 2^20 rows 54 against 57).
+inline bool sort_clears(int64_t n, int64_t rows, int64_t words) {
+  const int64_t blocks = n <= kSmall ? cluster_blocks(n) : sort_plan(n, rows).blocks;
+  return words <= (blocks + 1) << 15;
+}
+
 // Sorts into order[n]; workspace of sort_plan(n, rows).bytes() (none for few
 // tokens).
 inline cudaError_t sort_tokens(int64_t n, const Index& index, uint2* order, void* workspace,
                                const Fill& fill, cudaStream_t stream) {
-  // As many blocks as give each thread one token, then more tokens a thread.
-  if (n <= kSmall / 4) return cluster_sort<1>(n, index, order, fill, stream);
-  if (n <= kSmall / 2) return cluster_sort<2>(n, index, order, fill, stream);
-  if (n <= kSmall) return cluster_sort<4>(n, index, order, fill, stream);
+  if (n <= kSmall) {
+    switch (cluster_items(n)) {
+      case 1: return cluster_sort<1>(n, index, order, fill, stream);
+      case 2: return cluster_sort<2>(n, index, order, fill, stream);
+      default: return cluster_sort<4>(n, index, order, fill, stream);
+    }
+  }
   const SortPlan p = sort_plan(n, index.rows);
   switch (p.items) {
     case 2: return large_sort<2>(n, index, p, order, workspace, fill, stream);

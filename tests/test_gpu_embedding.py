@@ -1052,3 +1052,22 @@ def test_rows_wider_than_the_gpu_has_places(cuda, dtype, p):
             assert np.array_equal(ones[129, -1000:].cpu().numpy(), kept / (1 - p))
             terms = terms * ones
         assert torch.equal(got, _sums(terms, index, rows).to(dtype))
+
+
+@pytest.mark.parametrize("n,borders", [(300, (65_536,)), (2000, (98_304,)),
+                                       (8000, (294_912,)), (70_000, (1_179_648,))])
+def test_slots_cleared_by_the_sort_or_before_it(cuda, n, borders):
+    """Adam's slots on both sides of where a launch of their own clears them, over
+    memory that is not zero: rows without tokens get no gradient."""
+    import embedding
+
+    for rows in [r + more for r in borders for more in (0, 1)]:
+        index = torch.randint(0, rows, (n,), device=cuda,
+                              generator=torch.Generator(device=cuda).manual_seed(rows))
+        grad = torch.randint(1, 5, (n, 4), device=cuda,
+                             generator=torch.Generator(device=cuda).manual_seed(n)).float()
+        table, first, second = (torch.zeros(rows, 4, device=cuda) for _ in range(3))
+        torch.full((rows * 8 + n * 64,), 1.0, device=cuda)  # what the workspace held
+        embedding.consume_torch_adam(table, first, second, grad, index, rate=0.1, bias1=0.5,
+                                     bias2_sqrt=0.5)
+        assert torch.equal(first, ((1.0 - 0.9) * _sums(grad.double(), index, rows)).float())
