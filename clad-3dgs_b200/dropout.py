@@ -38,14 +38,16 @@ def _require(condition, message):
 def check_draw(p, seed, offset, device):
     """Checks a dropout's numbers; returns (offset as an int, address of the
     device offset or None)."""
-    _require(isinstance(p, (int, float)) and 0.0 <= p <= 1.0, "p must lie in [0, 1]")
-    _require(isinstance(seed, int) and 0 <= seed < WORD, "seed must be an integer in [0, 2^64)")
+    if not (isinstance(p, (int, float)) and 0.0 <= p <= 1.0):
+        raise RuntimeError("p must lie in [0, 1]")
+    if not (isinstance(seed, int) and 0 <= seed < WORD):
+        raise RuntimeError("seed must be an integer in [0, 2^64)")
     if isinstance(offset, torch.Tensor):
         _require(offset.device == device and offset.dtype == torch.int64
                  and offset.numel() == 1, "a tensor offset must be one int64 on the input's device")
         return 0, offset.data_ptr()
-    _require(isinstance(offset, int) and 0 <= offset < WORD,
-             "offset must be an integer in [0, 2^64) or a CUDA tensor")
+    if not (isinstance(offset, int) and 0 <= offset < WORD):
+        raise RuntimeError("offset must be an integer in [0, 2^64) or a CUDA tensor")
     return offset, None
 
 
