@@ -58,7 +58,7 @@ __device__ __forceinline__ Vec<T, V> finish(const Vec<T, V>& x, const bool (&kee
 // the output, whatever rows they belong to, so that stores are whole lines, U of
 // them each, all asked for before the first is stored. 1.1M rows of 48 floats
 // from 4096: 39 us (5.5 TB/s; groups of lanes a row 50, one vector a thread
-// 147); 16384 of 2048 bf16 from 131072: 20 us (6.8 TB/s).
+// 147); 16384 of 2048 bf16 from 131072, of which they name 6900: 20 us (4.8 TB/s).
 template <class T, class Division, int V, int U, bool kDrop>
 __global__ void __launch_bounds__(kThreads)
     lookup_kernel(typename Division::Number total, const Division vectors,

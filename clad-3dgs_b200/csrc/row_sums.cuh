@@ -52,7 +52,8 @@ constexpr uint32_t kNoRow = ~0u;
 // Rows a thread asks for at once (of each it takes `bytes`), and the blocks that
 // an SM's registers hold (200000 rows of 256 floats, 64 bytes a thread and row: 47
 // us with two blocks, 51 with three; 1M of 48 bf16, 32 bytes: 56 with three, 58 with
-// two).
+// two, although with three the kernels of two 16-bit vectors a lane spill 28 to 38
+// bytes a thread).
 constexpr int rows_at_once(int bytes, bool loose) {
   return loose ? 2 : bytes <= 8 ? 8 : bytes <= 16 ? 4 : 2;
 }
@@ -626,7 +627,8 @@ __global__ void __launch_bounds__(kThreads)
 // One launch for all of it: what counts at these sizes is the host's time for
 // each launch (2.3 us) and the workspace. Every block ranks the few tokens by
 // comparing each with all, then eight lanes share the tokens of a vector of the
-// table and add up in a fixed tree. A call on 37 tokens and 1000 x 45 f32 takes
+// table and add up in a fixed tree, in 32 bits (32 terms a lane at most and three
+// joins: 35 roundings). A call on 37 tokens and 1000 x 45 f32 takes
 // 11 us instead of 17, Adam of 60 x 48 with 184 tokens 13 instead of 22.
 //
 // The GPU's time must stay below the host's as well: at 128 tokens 5 us for 1365

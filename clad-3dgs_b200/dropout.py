@@ -15,8 +15,11 @@ it. It must not change between a forward pass and its backward pass (autograd
 checks the tensor's version).
 
 float32, float16 and bfloat16; inputs may have any layout, outputs are
-contiguous. Kernels launch on the current stream of x's device. Bad arguments
-raise RuntimeError before anything is written.
+contiguous. Kernels launch on the current stream of x's device and may be
+captured into a graph. (Torch cannot capture any backward pass while an eager
+autograd graph over the same leaf is alive: drop its outputs first, or capture
+`apply` on the gradient.) Bad arguments raise RuntimeError before anything is
+written.
 """
 
 from __future__ import annotations

@@ -20,8 +20,8 @@ Indices are int32 or int64, of any shape. A token equal to `padding_index`
 names no row: its output is zero and it gives no gradient. An index outside
 [0, rows) is treated the same and sets bit 256 of `_native.fault_status()` on
 the tensors' device (the calls do not synchronise to look; the reader, with
-that device current, does). Sums run in 32-bit floats in a fixed
-order: equal inputs give equal bits.
+that device current, does). Sums run in 32-bit floats in a fixed order (in 64
+bits where the parts of a very long row meet): equal inputs give equal bits.
 
 Kernels launch on the current stream of the tensors' device and may be captured
 into a graph. (Torch cannot capture any backward pass while an eager autograd
