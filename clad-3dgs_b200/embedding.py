@@ -179,7 +179,9 @@ def lookup_gradient(grad, index, rows, *, scale=1.0, padding_index=None, p=0.0, 
                     offset=0, order=None):
     """The table's gradient [rows, width] (grad's type) of a `lookup` with these
     arguments whose output has the gradient `grad` [*index.shape, width]. With
-    `order` (from `token_order`), index and padding_index are not read."""
+    `order` (from `token_order`), index and padding_index are not read. Not
+    recorded for reverse mode (its result does not require grad); a tangent in
+    forward mode goes through."""
     if forward_ad._current_level >= 0 and (parts := parts_of(grad)):  # as in lookup
         how = dict(scale=scale, padding_index=padding_index, p=p, seed=seed, offset=offset,
                    order=order)
