@@ -267,7 +267,7 @@ cudaError_t cluster_sort(int64_t n, const Index& index, uint2* order, const Fill
 
 // ---- many blocks ----
 
-constexpr int kSortBlocks = 148;
+constexpr int kSortBlocks = 148;  // a number of its own: it sets the workspace's size
 
 struct SortPlan {
   int items;         // tokens of a thread in a tile

@@ -250,7 +250,10 @@ class _Lookup(torch.autograd.Function):
         tensor = isinstance(offset, torch.Tensor)
         ctx.numbers = (table.shape[0], scale, padding_index, p, seed, None if tensor else offset,
                        order)
-        ctx.save_for_backward(index, *((offset,) if tensor else ()))
+        # An order's pairs are only saved to have their version checked (inference
+        # tensors have none).
+        ctx.save_for_backward(index, offset if tensor else None, None if order is None
+                              or order.pairs.is_inference() else order.pairs)
         return out
 
     @staticmethod
@@ -258,9 +261,9 @@ class _Lookup(torch.autograd.Function):
         if torch.is_grad_enabled():
             raise RuntimeError("embedding lookup supports first-order backward only")
         rows, scale, padding_index, p, seed, offset, order = ctx.numbers
-        index, *tensor = ctx.saved_tensors
+        index, tensor, _ = ctx.saved_tensors
         return (lookup_gradient(grad, index, rows, scale=scale, padding_index=padding_index, p=p,
-                                seed=seed, offset=tensor[0] if tensor else offset, order=order),
+                                seed=seed, offset=offset if tensor is None else tensor, order=order),
                 None, None, None, None, None, None, None)
 
 

@@ -1071,3 +1071,22 @@ def test_slots_cleared_by_the_sort_or_before_it(cuda, n, borders):
         embedding.consume_torch_adam(table, first, second, grad, index, rate=0.1, bias1=0.5,
                                      bias2_sqrt=0.5)
         assert torch.equal(first, ((1.0 - 0.9) * _sums(grad.double(), index, rows)).float())
+
+
+def test_an_order_written_before_the_backward_is_refused(cuda):
+    """As an index written after the forward pass is; an order of inference mode
+    has no version and is taken as it is."""
+    import embedding
+
+    table, index, grad = _case(700, 90, 48, torch.float32, cuda)
+    table.requires_grad_(True)
+    want = embedding.lookup_gradient(grad, index, 90)
+    with torch.inference_mode():
+        order = embedding.token_order(index, 90)
+    (got,) = torch.autograd.grad(embedding.lookup(table, index, order=order), table, grad)
+    assert torch.equal(got, want)
+    order = embedding.token_order(index, 90)
+    y = embedding.lookup(table, index, order=order)
+    order.pairs.copy_(embedding.token_order(index.flip(0).contiguous(), 90).pairs)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y, table, grad)
